@@ -149,11 +149,12 @@ Tensor bias_act(const Tensor& z, const Opt& bias, int64_t act, bool save8) {
 
 // --- FC layer on a kept input ----------------------------------------------
 
+// bf16 or fp32 (which holds what other types have beyond bf16)
 Tensor weight_view(const Tensor& w) {
   const auto t = w.scalar_type();
   return rows_view(t == torch::kBFloat16 || t == torch::kFloat32
                        ? w
-                       : w.detach().to(torch::kBFloat16));
+                       : w.detach().to(torch::kFloat32));
 }
 
 std::vector<int64_t> with_last(const Tensor& t, int64_t n) {

@@ -355,7 +355,7 @@ void linear8_fwd(const Tensor& x, const Tensor& w, const Opt& bias,
   TORCH_CHECK(W.K == cx.C, "linear8 shape mismatch");
   check_tiles(cx.rows, W.N);
   const Call cy(cx, W.N);
-  Tensor ws = cx.ws(yams::linear8_ws(cx.rows, W.N, W.K));
+  Tensor ws = cx.ws(yams::linear8_ws(cx.rows, W.N, W.K, W.dt));
   const bool narrow =
       bias.has_value() && bias->scalar_type() == torch::kBFloat16;
   yams::linear8_fwd(cx.in(x, "x"), W.dt, W.rows, narrow ? kBf16 : kF32,
@@ -371,7 +371,7 @@ void linear8_dgrad(const Tensor& dy, const Tensor& w, const Tensor& dx) {
   TORCH_CHECK(W.N == cy.C, "linear8 shape mismatch");
   check_tiles(cy.rows, W.K);
   const Call cx(cy, W.K);
-  Tensor ws = cx.ws(yams::linear8_ws(cx.rows, W.K, W.N));
+  Tensor ws = cx.ws(yams::linear8_ws(cx.rows, W.K, W.N, W.dt));
   yams::linear8_dgrad(cy.in(dy, "dy"), W.dt, W.rows, cx.out(dx, "dx"),
                       ws_ptr(ws), cx.rows, W.N, W.K, stream_of(dy));
 }
@@ -399,7 +399,7 @@ void linear8_wgrad(const Tensor& dy, const Tensor& codes, const Tensor& exps,
                      exps.data_ptr<uint8_t>()};
   const bool padded =
       int64_t(codes.storage().nbytes()) - codes.storage_offset() >= M * K + 7;
-  Tensor ws = cy.ws(yams::linear8_ws(cy.C, K, M));
+  Tensor ws = cy.ws(yams::linear8_ws(cy.C, K, M, kBf16));
   yams::linear8_wgrad(cy.in(dy, "dy"), x, padded, odt, dw.data_ptr(),
                       ws_ptr(ws), M, cy.C, int(K), stream_of(dy));
 }

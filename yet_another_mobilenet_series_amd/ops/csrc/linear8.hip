@@ -14,7 +14,7 @@
 // 4096: dw 818 us).  With one wave nothing but its own order hides latency:
 //   - tiles go global -> registers -> LDS.  Registers hold step t + 1 and
 //     then t + 2 while LDS holds t: a load has a step to arrive, and the
-//     way through registers decodes 8-bit codes and rounds fp32 weights.
+//     way through registers decodes 8-bit codes and splits fp32 weights.
 //   - a step is four quarters of 16 along k.  While a quarter's MFMAs run,
 //     the fragments of the next one are read, and in the first three the
 //     next step is stored to the other buffer.  The only barrier of a step
@@ -30,8 +30,13 @@
 // A long reduction with few output tiles is split; the splits leave fp32
 // slabs that a second kernel adds in a fixed order.
 //
-// fp32 weights are rounded to bf16 on the way, as the matrix unit takes them:
-// off by 2^-8 of each weight at most, as in `linear` without codes.
+// fp32 weights w go to the matrix unit as two bf16 values, their upper half
+// and the rounded rest, in two passes over k that add to the same
+// accumulators: what is left out is at most 2^-15 of w (rounded once they
+// would be off by 2^-8, which is seen in y and dx: those are rounded to bf16,
+// by 2^-8 too).  fp16 weights are exact so.  It costs the second pass: 16384
+// rows, 4096 x 4096 weights in fp32: y 1130 us, dx 1180 (rounded once: 535 and
+// 560), 256 rows, 1280 x 1000: 16 and 18 with the join of splits (12 and 10).
 //
 // Measured (16384 rows, 4096 x 4096 weights, bf16): y 450 us (1222 TFLOP/s),
 // dx 479 (1148), dw 570 (965); the library's products, without codes, 357,
@@ -94,20 +99,32 @@ struct Staged {
     if constexpr (KIND == OP_CODE)
       exponent = n > 0 ? o.exps[row * o.G + (col >> 5)] : 0u;
   }
+  // PART, of fp32: 0 the upper halves (truncated, so that nothing finite
+  // becomes infinite), 1 what they leave; infinities leave nothing
+  template <int PART>
   DEV_INLINE uint4_t bf16() const {
+    uint4_t r;
     if constexpr (KIND == OP_BF16) {
       return w;
+    } else if constexpr (KIND == OP_F32 && PART == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
+      return r;
     } else {
       float v[8];
       if constexpr (KIND == OP_F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+        for (int e = 0; e < 8; ++e)
+          v[e] = (w[e] & 0x7fffffffu) == 0x7f800000u
+                     ? 0.f
+                     : __uint_as_float(w[e]) -
+                           __uint_as_float(w[e] & 0xffff0000u);
       } else {
         const float unit = exp_unit(exponent);
         dequantize4(w[0], unit, v);
         dequantize4(w[1], unit, v + 4);
       }
-      uint4_t r;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         r[e] = unsigned(f2bf(v[2 * e])) | unsigned(f2bf(v[2 * e + 1])) << 16;
@@ -184,10 +201,10 @@ struct Side {
   }
 
   // MASK: the step's k from z on become zero
-  template <bool MASK = false>
+  template <int PART, bool MASK = false>
   DEV_INLINE void store(ushort_t* lds, int c, int z = 0) const {
     const int tid = int(threadIdx.x);
-    uint4_t v = st[c].bf16();
+    uint4_t v = st[c].template bf16<PART>();
     int at;
     if constexpr (!ACROSS) {
       const int i = (tid >> 3) + kRows * c, k = (tid & 7) * 8;
@@ -329,22 +346,24 @@ __global__ __launch_bounds__(256, S::F > 2 ? 1 : 2) void product_kernel(
       }
     }
   };
-  auto store = [&](int t, int c0, int c1) {
+  auto store = [&](auto part, int t, int c0, int c1) {
+    constexpr int P = decltype(part)::value;
     ushort_t* buf = lds + (t & 1) * kBuf;
 #pragma unroll
     for (int c = c0; c < c1; ++c)
       if (c < SA::N)
-        a.store(buf, c);
+        a.template store<P>(buf, c);
       else
-        b.store(buf + SA::kElems, c - SA::N);
+        b.template store<P>(buf + SA::kElems, c - SA::N);
   };
-  auto store_first = [&]() {
+  auto store_first = [&](auto part) {
+    constexpr int P = decltype(part)::value;
     const int z = int(k1 - k0) - (steps - 1) * TK;
 #pragma unroll
-    for (int c = 0; c < SA::N; ++c) a.template store<true>(lds, c, z);
+    for (int c = 0; c < SA::N; ++c) a.template store<P, true>(lds, c, z);
 #pragma unroll
     for (int c = 0; c < SB::N; ++c)
-      b.template store<true>(lds + SA::kElems, c, z);
+      b.template store<P, true>(lds + SA::kElems, c, z);
   };
   bf16x8 fa[2][F], fb[2][F];
   // fragment f of quarter h: B's, which its first MFMAs all need, then A's
@@ -375,12 +394,12 @@ __global__ __launch_bounds__(256, S::F > 2 ? 1 : 2) void product_kernel(
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  if (steps > 0) {
+  auto walk = [&](auto part) {
     load(0, 0, NC);
     if (FAST)
-      store_first();
+      store_first(part);
     else
-      store(0, 0, NC);
+      store(part, 0, 0, NC);
     // in the order of the loop, whose waits count on it
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -397,7 +416,7 @@ __global__ __launch_bounds__(256, S::F > 2 ? 1 : 2) void product_kernel(
         read(t, h + 1, 2 * r);
         read(t, h + 1, 2 * r + 1);
         multiply(h, r);
-        store(t + 1, NC * x / (3 * F), NC * (x + 1) / (3 * F));
+        store(part, t + 1, NC * x / (3 * F), NC * (x + 1) / (3 * F));
         load(t + 2, NC * x / (3 * F), NC * (x + 1) / (3 * F));
         interleave();
       }
@@ -417,6 +436,15 @@ __global__ __launch_bounds__(256, S::F > 2 ? 1 : 2) void product_kernel(
 #pragma unroll
       for (int r = R + 1; r < F; ++r) multiply(3, r);
       __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (steps > 0) {
+    walk(std::integral_constant<int, 0>{});
+    if constexpr (KB == OP_F32) {
+      lds_barrier();  // the buffers are still being read
+      // the first pass is not to keep what this one can find again
+      asm volatile("" : "+s"(A.p), "+s"(B.p));
+      walk(std::integral_constant<int, 1>{});
     }
   }
 
@@ -518,7 +546,8 @@ struct Plan {
 // FAST: tiles and steps are whole or can be shifted so that they are
 // (`loose`: codes without readable bytes behind them cannot be).  The
 // largest tile exists only so: its registers have no room for checks.
-Plan plan_of(int64_t I, int64_t J, int64_t K, bool loose) {
+// `passes` over k: two for fp32 weights.
+Plan plan_of(int64_t I, int64_t J, int64_t K, int passes, bool loose) {
   Plan best{};
   double least = 0.0;
   for (const Tile& tile : kTiles) {
@@ -542,7 +571,7 @@ Plan plan_of(int64_t I, int64_t J, int64_t K, bool loose) {
           tile.most == 1 ? tile.one
                          : tile.one + (tile.full - tile.one) * (held - 1) /
                                           (tile.most - 1);
-      double t = rounds * (tile.base + step * double(p.per / TK) *
+      double t = rounds * (tile.base + step * double(p.per / TK * passes) *
                                            (p.fast ? 1.0 : 1.5));
       if (p.splits > 1) t += 4.0 + 8.0 * I * J * p.splits / 4.5e6;
       if (best.W == 0 || t < least) {
@@ -569,7 +598,7 @@ void launch(const Plan& p, Operand A, Operand B, bool bf16, void* C,
 template <int KA, bool XA, int KB, bool XB>
 void product(Operand A, Operand B, int odt, void* C, Bias bias, float* ws,
              int64_t I, int64_t J, int64_t K, bool loose, hipStream_t s) {
-  const Plan p = plan_of(I, J, K, loose);
+  const Plan p = plan_of(I, J, K, KB == OP_F32 ? 2 : 1, loose);
   const bool split = p.splits > 1, bf16 = odt == DT_BF16 && !split;
   void* to = split ? ws : C;
   const Bias add = split ? Bias{} : bias;
@@ -668,11 +697,12 @@ Operand operand(RowsDesc r) { return {r.p, r.stride, nullptr, 0}; }
 
 }  // namespace
 
-int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth) {
+int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth, int wdt) {
   if (rows == 0 || cols == 0 || depth == 0) return 0;
   int64_t most = 0;  // of the two plans that the product may have
   for (const bool loose : {false, true}) {
-    const int splits = plan_of(rows, cols, depth, loose).splits;
+    const int splits =
+        plan_of(rows, cols, depth, wdt == DT_F32 ? 2 : 1, loose).splits;
     if (splits > 1) most = std::max(most, splits * rows * cols);
   }
   return most;

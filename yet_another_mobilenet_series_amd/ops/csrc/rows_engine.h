@@ -83,7 +83,7 @@ int64_t join_bwd_ws(int dt, const JoinDesc& d);  // floats of `ws`
 
 // --- FC layer on a kept input (linear8.hip) -------------------------------
 // Row-major operands with any row stride.  `wdt`: DT_BF16 or DT_F32 (which
-// is rounded to bf16 on its way in); out types DT_BF16 or DT_F32.
+// goes in as two bf16 parts); out types DT_BF16 or DT_F32.
 // y[M, N] = x[M, K] w[N, K]^T + bias; `bdt`: the bias, DT_BF16 or DT_F32
 void linear8_fwd(RowsDesc x, int wdt, RowsDesc w, int bdt, const void* bias,
                  void* y, float* ws, int64_t M, int N, int K, hipStream_t s);
@@ -94,8 +94,9 @@ void linear8_dgrad(RowsDesc dy, int wdt, RowsDesc w, void* dx, float* ws,
 // behind the codes may be read
 void linear8_wgrad(RowsDesc dy, Kept x, bool padded, int odt, void* dw,
                    float* ws, int64_t M, int N, int K, hipStream_t s);
-// floats of `ws` for [rows, cols] outputs over a reduction of `depth`
-int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth);
+// floats of `ws` for [rows, cols] outputs over a reduction of `depth`; `wdt`
+// of the weights (the weight gradient has codes in their place: DT_BF16)
+int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth, int wdt);
 // db = sum over rows of dy; ws of row_sum_ws floats; db as dbias above
 // (`odt` DT_F32) or bf16 [C] (DT_BF16)
 void row_sum(int dt, RowsDesc dy, int odt, void* db, float* ws, int64_t rows,

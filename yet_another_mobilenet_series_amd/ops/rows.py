@@ -340,8 +340,8 @@ def linear8(x: torch.Tensor, weight: torch.Tensor,
             save8: bool = True) -> torch.Tensor:
     """``linear`` with ``save8``: ``act(x @ weight.T + bias)`` over the last
     axis of x; x, and z = x @ weight.T where there is an activation, are
-    kept in 8 bits.  GPU: bf16 in and out (like ``linear``, other dtypes are
-    rounded to it)."""
+    kept in 8 bits.  GPU: bf16 in and out (like ``linear``, rows of other
+    dtypes are rounded to it); weights count with 15 bits and more."""
     _check_rows(x, "x")
     if (x.dim() > 2 and weight.dim() == 2 and x.shape[-1] != weight.shape[1]
             and x.shape[1:].numel() == weight.shape[1]):
