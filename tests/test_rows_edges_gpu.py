@@ -71,3 +71,63 @@ def test_linear_keeps_infinite_and_largest_weights_apart(m, k, n):
     want = (x.double() * 2.0 ** -10) @ w[rest].double().t()
     assert bool((y[:, rest].double() - want).abs().le(
         2.0 ** -7 * want.abs() + 1e-6).all())
+
+
+# ---------------------------------------------------------------------------
+# infinities in rows kept in 8 bits
+# ---------------------------------------------------------------------------
+
+def _same(a, b):
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(
+        a.nan_to_num(7.0, 8.0, 9.0), b.nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("shape,shared", [
+    # short last chunks, teams without a row, rows of several waves
+    ((3, 5), False), ((3, 20), False), ((3, 32), False), ((2, 3, 333), False),
+    ((9, 4104), False), ((5, 3, 20), True), ((70, 5, 64), True),
+    ((3, 3, 333), True)])
+@pytest.mark.parametrize("where", ["gates closed", "gates open or closed",
+                                   "h", "x"])
+def test_infinities_in_kept_rows_stay_where_they_are(dtype, kind, shape,
+                                                     shared, where):
+    """The gradient is the one of the same call on the unpacked values, NaN
+    and infinities included: nothing comes from channels behind the last one
+    or from threads without a row."""
+    c, inf = shape[-1], float("inf")
+    h, x = _rand(1, *shape, dtype=dtype), _rand(2, *shape, dtype=dtype)
+    g = _rand(3, *((shape[0], c) if shared else shape), dtype=dtype)
+    if where == "gates closed":
+        g.fill_(-inf)
+    elif where == "gates open or closed":
+        g[0] = torch.where(torch.arange(c, device=DEV) % 2 == 0, inf, -inf)
+    else:
+        (h if where == "h" else x).view(-1, c)[0, -1] = inf
+    w, s, w2 = (_rand(i, c) for i in (5, 6, 7))
+    b = _rand(8, c) if kind == "layer" else None
+    dy, du = _rand(9, *shape, dtype=dtype), _rand(10, *shape, dtype=dtype)
+
+    def grads(h, x, g, save8, post):
+        leaves = [t.detach().clone().requires_grad_()
+                  for t in (h, x, g, s, w2) + ((w,) if post else ())]
+        outs = ops.norm_residual(
+            leaves[0], leaves[1], leaves[5] if post else None,
+            b if post else None, gate=leaves[2], gate_act="sigmoid",
+            scale=leaves[3], post_norm=post, next_norm=True,
+            next_weight=leaves[4], next_bias=b, kind=kind, save8=save8)
+        return (torch.autograd.grad(outs[0], leaves[:4], dy,
+                                    retain_graph=True)
+                + torch.autograd.grad(outs, leaves, [dy, du]))
+
+    def at(t):
+        return ops.pack_activation(t).unpack()
+
+    for post in (True, False):
+        got = grads(h, x, g, True, post)
+        want = grads(at(h), at(x), at(g), False, post)
+        for k, (p, q) in enumerate(zip(got, want)):
+            assert _same(p, q), (post, k)
+            if where.startswith("gates"):
+                assert bool(p.isfinite().all()), (post, k)

@@ -243,6 +243,16 @@ join_bwd_kernel(
     }
   };
 
+  // `n_` (0..8) of the chunk's values, and zeros: what lies behind the last
+  // channel has code 0, which is NaN in a group with a non-finite value
+  auto decode = [&](const RawChunk<DT, KEPT>& q, int n_, float* v) {
+    q.decode(v);
+    if (KEPT && p.read != READ_WHOLE) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n_ ? v[e] : 0.f;
+    }
+  };
+
   // this block's runs of rows
   int64_t run0, run1;
   int part = 0;
@@ -268,7 +278,7 @@ join_bwd_kernel(
              p.read == READ_SHORT ? n[j] : -1);
         if (p.read == READ_RAGGED) q.drop(n[j]);
         q.blank(n[j]);
-        q.decode(gs[j]);
+        decode(q, n[j], gs[j]);
       }
       gate_prepare<NV>(gs, p.gate_act);
     }
@@ -302,8 +312,8 @@ join_bwd_kernel(
       if constexpr (HAS_H) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          cur.h[j].decode(h[j]);
-          if constexpr (GATE == GATE_FULL) cur.g[j].decode(g[j]);
+          decode(cur.h[j], n[j], h[j]);
+          if constexpr (GATE == GATE_FULL) decode(cur.g[j], n[j], g[j]);
         }
         if constexpr (GATE == GATE_FULL) gate_prepare<NV>(g, p.gate_act);
         float mean = 0.f;
@@ -320,7 +330,7 @@ join_bwd_kernel(
       if (next) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          cur.x[j].decode(x[j]);
+          decode(cur.x[j], n[j], x[j]);
           if constexpr (HAS_H) {
             float w[8], s[8], b[8] = {};
             pw.get(p.w, t + j * TPR, n[j], 1.f, 1.f, w);

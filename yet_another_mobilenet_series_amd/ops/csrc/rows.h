@@ -437,7 +437,11 @@ struct RawChunk {
   }
   // what load() has read of a chunk of n (0..8)
   DEV_INLINE void drop(int n) { w = drop_words<kSize>(w, n > 0 ? 8 - n : 0); }
-  DEV_INLINE void blank(int n) { w = n > 0 ? w : Words<kSize>(0u); }
+  // (its group too: code 0 of a group with a non-finite value is NaN)
+  DEV_INLINE void blank(int n) {
+    w = n > 0 ? w : Words<kSize>(0u);
+    if constexpr (KEPT) exponent = n > 0 ? exponent : 0u;
+  }
   DEV_INLINE void load_exponent(const unsigned char* base, unsigned off) {
     exponent = *lane_at<unsigned char>(base, off);
   }
