@@ -131,3 +131,34 @@ def test_infinities_in_kept_rows_stay_where_they_are(dtype, kind, shape,
             assert _same(p, q), (post, k)
             if where.startswith("gates"):
                 assert bool(p.isfinite().all()), (post, k)
+
+
+@pytest.mark.parametrize("save8", [False, True])
+@pytest.mark.parametrize("post", [False, True])
+def test_infinite_shared_gates_add_nothing_without_a_row(save8, post):
+    """Three rows a run, threads for more: sums over the rows are those of
+    the three.  (Without a norm behind it y may be infinite.)"""
+    c = 40
+    h, x = _rand(1, 4, 3, c).abs() + 0.5, _rand(2, 4, 3, c)
+    g = _rand(3, 4, c)
+    g[1, :32] = float("inf")
+    s = _rand(4, c).requires_grad_()
+    w = (_rand(5, c).abs() + 0.5).requires_grad_() if post else None
+    dy = _rand(6, 4, 3, c).abs() + 0.5
+    y = ops.norm_residual(h, x, w, gate=g, scale=s, post_norm=post,
+                          save8=save8)
+    got = torch.autograd.grad(y, [s] + ([w] if post else []), dy)
+    h64, g64 = h.double(), g.double()
+    if save8:
+        h64 = ops.pack_activation(h).unpack().double()
+        g64 = ops.pack_activation(g).unpack().double()
+    s64 = s.detach().double().requires_grad_()
+    w64 = w.detach().double().requires_grad_() if post else None
+    n = h64 / (h64.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w64 \
+        if post else h64
+    want = torch.autograd.grad((s64 * g64[:, None] * n * dy.double()).sum(),
+                               [s64] + ([w64] if post else []))
+    for p, q in zip(got, want):
+        assert torch.equal(p.isnan(), q.isnan())
+        assert torch.equal(p.isinf(), q.isinf())
+        assert torch.equal(p[:32].sign(), q[:32].sign().float())

@@ -298,7 +298,8 @@ join_bwd_kernel(
           for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(gs[j][e]));
       }
       const bool live = base + team < hi;
-      // A team without a row has zeros, and r = ry = 0: it adds nothing.
+      // A team without a row has zeros, and r = ry = 0: it adds nothing (its
+      // shared gates are the run's, and may be infinite: they are left out).
       int m_[NV];  // channels to store
       float dY[NV][8], x[NV][8], h[NV][8], g[NV][8];
 #pragma unroll
@@ -433,6 +434,7 @@ join_bwd_kernel(
             const float d = dY[j][e];
             const float nn =
                 LAYER ? fmaf(h[j][e], w[e], b[e]) : h[j][e] * w[e];
+            if (SHARED) a = live ? a : 0.f;
             const float ga = GATE != GATE_NONE ? d * a : d;
             if (GATE != GATE_NONE) g[j][e] = d * s[e] * da * nn;
             a_t[j][e] = fmaf(ga, h[j][e], a_t[j][e]);
