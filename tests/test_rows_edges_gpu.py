@@ -162,3 +162,22 @@ def test_infinite_shared_gates_add_nothing_without_a_row(save8, post):
         assert torch.equal(p.isnan(), q.isnan())
         assert torch.equal(p.isinf(), q.isinf())
         assert torch.equal(p[:32].sign(), q[:32].sign().float())
+
+
+# ---------------------------------------------------------------------------
+# forward-mode derivatives
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("save8", [False, True])
+def test_tangents_are_refused(save8):
+    from torch.autograd import forward_ad
+    x, w = _rand(1, 4, 8), _rand(2, 8, 8)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.row_norm(d, save8=save8),
+                     lambda: ops.bias_act(d, None, "relu", save8),
+                     lambda: ops.norm_residual(x, d, save8=save8),
+                     lambda: ops.norm_residual(x, x, gate=d, save8=save8),
+                     lambda: ops.linear(d, w, None, save8=True)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

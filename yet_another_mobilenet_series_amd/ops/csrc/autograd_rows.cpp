@@ -85,7 +85,12 @@ Tensor like(const Tensor& t) {  // contiguous, of its shape and type
   return torch::empty(t.sizes(), t.options());
 }
 
+// A tangent is refused here: the kernels would drop it, and an output without
+// one counts as a constant.
 bool wants_grad(std::initializer_list<Tensor> ts) {
+  for (const Tensor& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                "the row operators have no forward-mode derivative");
   if (!torch::GradMode::is_enabled()) return false;
   for (const Tensor& t : ts)
     if (t.defined() && t.requires_grad()) return true;
