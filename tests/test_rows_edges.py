@@ -48,3 +48,34 @@ def test_tangents_pass_through_the_reference():
     want = (ops.row_norm((x + a * t).double())
             - ops.row_norm((x - a * t).double())) / (2 * a)
     assert torch.allclose(u.tangent.double(), want, atol=1e-4)
+
+
+# ---------------------------------------------------------------------------
+# sizes
+# ---------------------------------------------------------------------------
+
+def test_the_context_leaves_what_the_codec_does_not_take(monkeypatch):
+    """A tensor of too many chunks, or a layer of too many inputs, is handled
+    as without the context instead of ending the forward pass."""
+    one = torch.empty(1)
+    assert R._fits(one.expand((1 << 29) - 1, 1))
+    assert not R._fits(one.expand(1 << 29, 1))       # 4 chunks a row
+    assert not R._fits(one.expand(1 << 24, 1024))    # 128
+    assert R._fits(one.expand((1 << 24) - 1, 1024))
+    assert not R._fits(one.expand(1, 1 << 30))
+    monkeypatch.setattr(R, "_fits", lambda t: t.shape[-1] < 64)
+    x = torch.randn(4, 64)
+    w = torch.randn(64, 64, requires_grad=True)
+    with ops.activations_8bit(min_numel=1):
+        y = torch.tanh(x @ w)
+    got, = torch.autograd.grad(y.sum(), w)
+    want, = torch.autograd.grad(torch.tanh(x @ w).sum(), w)
+    assert torch.equal(got, want)
+
+    monkeypatch.setattr(R, "MAX_LINEAR_CHANNELS", 32)
+    x = x.requires_grad_()
+    with ops.activations_8bit(min_numel=1):
+        y = ops.linear(x, w)
+    got, = torch.autograd.grad(y.square().sum(), w)
+    want, = torch.autograd.grad(ops.linear(x, w).square().sum(), w)
+    assert torch.equal(got, want)

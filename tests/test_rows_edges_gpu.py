@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from yet_another_mobilenet_series_amd import ops
+from yet_another_mobilenet_series_amd.ops import rows as R
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +182,45 @@ def test_tangents_are_refused(save8):
                      lambda: ops.linear(d, w, None, save8=True)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+# ---------------------------------------------------------------------------
+# sizes
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("view", ["whole", "far apart"])
+def test_rows_of_more_than_2_to_22_channels(dtype, view):
+    far = (1 << 22) + 8
+    x = _rand(3, 3, far, dtype=dtype)
+    if view == "far apart":
+        x = x[:, 5:1005]
+    c = x.shape[1]
+    p = ops.pack_activation(x)
+    codes, exps = R._ref_pack(x.cpu())
+    assert torch.equal(p.codes.cpu(), codes)
+    assert torch.equal(p.exponents.cpu(), exps)
+    assert torch.equal(p.unpack().cpu(), R._ref_unpack(codes, exps, dtype))
+    b = _rand(4, c).requires_grad_()
+    dy = _rand(5, 3, far, dtype=dtype)[:, :c]
+    for save8 in (True, False):
+        z = x.detach().requires_grad_()
+        y = ops.bias_act(z, b, "relu", save8=save8)
+        dz, db = torch.autograd.grad(y, [z, b], dy)
+        # one operation in fp32 and a rounding: the same bits
+        assert torch.equal(y, torch.relu(x.float() + b).to(dtype))
+        at = p.unpack() if save8 else x
+        want = torch.where(at.float() + b > 0, dy, 0)
+        assert torch.equal(dz, want)
+        _within(db, want.double().sum(0), 3 * U32 * dy.double().abs().sum(0))
+    with ops.activations_8bit():
+        z = x.detach().requires_grad_()
+        t = torch.tanh(z * 1.0)
+    dz, = torch.autograd.grad(t.sum(), z)
+    assert bool(dz.isfinite().all())
+    if view == "whole":
+        w = torch.zeros(1, c, dtype=dtype, device=DEV)
+        with pytest.raises(ValueError, match="at most"):
+            ops.linear(x, w, None, save8=True)
+    u = ops.row_norm(x[:, 8:1000])  # copied
+    assert torch.equal(u, ops.row_norm(x[:, 8:1000].contiguous()))

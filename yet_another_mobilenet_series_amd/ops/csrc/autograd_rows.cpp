@@ -18,22 +18,24 @@ using torch::autograd::Function;
 using torch::autograd::variable_list;
 typedef c10::optional<Tensor> Opt;
 
-constexpr int64_t kMaxStride = int64_t(1) << 22;
-
 Tensor plain(const Opt& t) { return t.has_value() ? *t : Tensor(); }
 Opt maybe(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 
-// [rows, C] with unit stride along C and rows that the kernels reach: a view
-// where there is one
-Tensor rows_view(const Tensor& x) {
+// [rows, C] with unit stride along C: a view where there is one
+Tensor any_rows(const Tensor& x) {
   const int64_t c = x.size(-1);
   Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / c, c});
-  if ((c == 1 || r.stride(1) == 1) &&
-      (r.size(0) <= 1 || r.stride(0) <= kMaxStride))
-    return r;
+  if (c == 1 || r.stride(1) == 1) return r;
   // (contiguous() leaves an empty tensor as it is)
   return r.numel() == 0 ? torch::empty(r.sizes(), r.options())
                         : r.contiguous();
+}
+
+// ... and rows that norms and products reach (longer ones they refuse)
+Tensor rows_view(const Tensor& x) {
+  Tensor r = any_rows(x);
+  return r.size(0) <= 1 || r.stride(0) <= yams::kMaxStride ? r
+                                                           : r.contiguous();
 }
 
 Opt rows_opt(const Tensor& x) {
@@ -119,7 +121,7 @@ Tensor bias_act_run(const Tensor& rows, const Tensor& z, const Tensor& bias,
 struct BiasActFn : Function<BiasActFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& z,
                         const Opt& bias_opt, int64_t act, bool keep) {
-    const Tensor rows = rows_view(z), bias = plain(bias_opt);
+    const Tensor rows = any_rows(z), bias = plain(bias_opt);
     Codes k;
     if (keep) k = empty_codes(rows);
     Tensor y = bias_act_run(rows, z, bias, act, k);
@@ -131,13 +133,13 @@ struct BiasActFn : Function<BiasActFn> {
     once();
     const variable_list s = ctx->get_saved_variables();
     const Tensor &z = s[0], &bias = s[3];
-    const Tensor rows = rows_view(dys[0]);
+    const Tensor rows = any_rows(dys[0]);
     const int64_t m = rows.size(0), c = rows.size(1);
     Tensor dz = like(dys[0]), sums, db;
     if (bias.defined() && ctx->needs_input_grad(1))
       sums = sums_of(rows, 1, m);
     if (m > 0)
-      act_rows_bwd(rows, rows_opt(z), maybe(s[1]), maybe(s[2]),
+      act_rows_bwd(rows, z.defined() ? Opt(any_rows(z)) : Opt(), maybe(s[1]), maybe(s[2]),
                    param32(bias), ctx->saved_data["act"].toInt(),
                    dz, maybe(sums));
     if (sums.defined()) db = sum_at(sums, 0, c, bias.scalar_type());
@@ -148,7 +150,7 @@ struct BiasActFn : Function<BiasActFn> {
 Tensor bias_act(const Tensor& z, const Opt& bias, int64_t act, bool save8) {
   const Tensor b = plain(bias);
   if (!wants_grad({z, b}))
-    return bias_act_run(rows_view(z), z, b, act, Codes());
+    return bias_act_run(any_rows(z), z, b, act, Codes());
   return BiasActFn::apply(z, bias, act, save8);
 }
 
@@ -400,7 +402,7 @@ std::vector<Tensor> join(const Opt& h, const Tensor& x, const Opt& gate,
 // --- codec -----------------------------------------------------------------
 
 std::pair<Tensor, Tensor> pack(const Tensor& x) {
-  const Tensor rows = rows_view(x.requires_grad() ? x.detach() : x);
+  const Tensor rows = any_rows(x.requires_grad() ? x.detach() : x);
   Codes k = empty_codes(rows);
   if (rows.size(0) > 0) pack_rows(rows, k.codes, k.exps);
   return {k.codes, k.exps};

@@ -18,6 +18,7 @@ using torch::Tensor;
 typedef c10::optional<Tensor> Opt;
 
 constexpr int kBf16 = 0, kF16 = 1, kF32 = 2;  // DT_* of rows.h
+using yams::kMaxStride;
 
 int dtype_of(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
@@ -38,14 +39,19 @@ float* ws_ptr(const Tensor& ws) {
   return ws.defined() ? ws.data_ptr<float>() : nullptr;
 }
 
+// How far apart a kernel takes rows: norms and products address the rows of a
+// block from a common base with 32 bits, the others every row with 64.
+enum Apart { NEAR, ANY };
+
 // the tensors of one call: one device, one row type, one shape
 struct Call {
   const Tensor& ref;
+  Apart apart;
   int dt;
   int64_t rows;
   int C;
 
-  Call(const Tensor& t, const char* name) : ref(t) {
+  Call(const Tensor& t, const char* name, Apart a = NEAR) : ref(t), apart(a) {
     TORCH_CHECK(t.is_cuda() && t.dim() == 2, name,
                 " must be [rows, C] on a GPU");
     dt = dtype_of(t, name);
@@ -57,7 +63,7 @@ struct Call {
 
   // other channels of the same rows
   Call(const Call& o, int channels)
-      : ref(o.ref), dt(o.dt), rows(o.rows), C(channels) {}
+      : ref(o.ref), apart(o.apart), dt(o.dt), rows(o.rows), C(channels) {}
 
   int64_t groups() const { return (int64_t(C) + 31) / 32; }
 
@@ -76,8 +82,7 @@ struct Call {
                 " has the wrong shape");
     TORCH_CHECK(C == 1 || t.stride(1) == 1, name,
                 " needs unit stride along the channels");
-    // lanes address up to 64 rows from a common base with 32 bits
-    TORCH_CHECK(want <= 1 || t.stride(0) <= (int64_t(1) << 22), name,
+    TORCH_CHECK(apart == ANY || want <= 1 || t.stride(0) <= kMaxStride, name,
                 ": rows are too far apart");
     return {t.data_ptr(), t.stride(0)};
   }
@@ -150,7 +155,7 @@ struct Call {
 }  // namespace
 
 void pack_rows(const Tensor& x, const Tensor& codes, const Tensor& exps) {
-  const Call c(x, "x");
+  const Call c(x, "x", ANY);
   c10::cuda::CUDAGuard guard(x.device());
   c.check_chunks();
   yams::pack_rows(c.dt, c.in(x, "x"), c.kept(codes, exps, "x"), c.rows, c.C,
@@ -158,7 +163,7 @@ void pack_rows(const Tensor& x, const Tensor& codes, const Tensor& exps) {
 }
 
 void unpack_rows(const Tensor& codes, const Tensor& exps, const Tensor& y) {
-  const Call c(y, "y");
+  const Call c(y, "y", ANY);
   c10::cuda::CUDAGuard guard(y.device());
   c.check_chunks();
   yams::unpack_rows(c.dt, c.kept(codes, exps, "y"), c.out(y, "y"), c.rows,
@@ -167,7 +172,7 @@ void unpack_rows(const Tensor& codes, const Tensor& exps, const Tensor& y) {
 
 void act_rows_fwd(const Tensor& z, const Opt& bias, int64_t act,
                   const Tensor& y, const Opt& codes, const Opt& exps) {
-  const Call c(z, "z");
+  const Call c(z, "z", ANY);
   c10::cuda::CUDAGuard guard(z.device());
   c.check_chunks();
   yams::act_rows_fwd(c.dt, c.in(z, "z"), c.param(bias, "bias"), int(act),
@@ -178,7 +183,7 @@ void act_rows_fwd(const Tensor& z, const Opt& bias, int64_t act,
 void act_rows_bwd(const Tensor& dy, const Opt& z, const Opt& codes,
                   const Opt& exps, const Opt& bias, int64_t act,
                   const Tensor& dz, const Opt& dbias) {
-  const Call c(dy, "dy");
+  const Call c(dy, "dy", ANY);
   c10::cuda::CUDAGuard guard(dy.device());
   TORCH_CHECK(z.has_value() != codes.has_value(),
               "act_rows_bwd takes z or its codes");
@@ -326,7 +331,7 @@ Weight weight_of(const Tensor& w, const Tensor& ref) {
   TORCH_CHECK(dt != kF16, "weight must be bf16 or fp32");
   TORCH_CHECK(w.dim() == 2 && (w.size(1) == 1 || w.stride(1) == 1),
               "weight must be [out, in] with unit stride along in");
-  TORCH_CHECK(w.size(0) <= 1 || w.stride(0) <= (int64_t(1) << 22),
+  TORCH_CHECK(w.size(0) <= 1 || w.stride(0) <= kMaxStride,
               "weight: rows are too far apart");
   TORCH_CHECK(w.size(0) < (int64_t(1) << 30) &&
                   w.size(1) < (int64_t(1) << 30),
@@ -405,7 +410,7 @@ void linear8_wgrad(const Tensor& dy, const Tensor& codes, const Tensor& exps,
 }
 
 void row_sum(const Tensor& dy, const Tensor& db) {
-  const Call c(dy, "dy");
+  const Call c(dy, "dy", ANY);
   c10::cuda::CUDAGuard guard(dy.device());
   Tensor ws = c.ws(yams::row_sum_ws(c.rows, c.C));
   const bool narrow = db.scalar_type() == torch::kBFloat16;

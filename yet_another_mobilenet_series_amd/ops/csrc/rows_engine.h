@@ -19,6 +19,10 @@ struct Kept {  // a kept activation; null pointers where there is none
   unsigned char* exps = nullptr;
 };
 
+// elements between rows where a kernel addresses up to 64 of them with 32
+// bits of bytes (norms and products)
+constexpr int64_t kMaxStride = int64_t(1) << 22;
+
 struct RowsDesc {
   const void* p = nullptr;
   int64_t stride = 0;

@@ -204,8 +204,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor,
     """FC layer (K10) with optional fused activation. weight: [out, in].
 
     ``save8`` keeps what the backward pass needs of the activations in 8
-    bits (:mod:`.rows`; default: as ``activations_8bit`` says)."""
-    if (rows.saving_8bit() if save8 is None else save8):
+    bits (:mod:`.rows`; default: as ``activations_8bit`` says, for layers
+    of the size that ``save8`` takes)."""
+    if save8 is None:
+        save8 = (rows.saving_8bit()
+                 and max(weight.shape) <= rows.MAX_LINEAR_CHANNELS)
+    if save8:
         return rows.linear8(x, weight, bias, act_code(act))
     if use_hip(x):
         return hip_ops.linear(x, weight, bias, act)

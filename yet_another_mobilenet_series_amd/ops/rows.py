@@ -47,6 +47,8 @@ _LEAST = {torch.float16: -24, torch.bfloat16: -126, torch.float32: -126}
 #: the unit of the dtype's top binade, where codes stop at 63
 _LAST = {torch.float16: 10, torch.bfloat16: 122, torch.float32: 122}
 MAX_NORM_CHANNELS = 16384
+#: inputs and outputs of an FC layer whose input is kept in 8 bits
+MAX_LINEAR_CHANNELS = 1 << 22
 
 _GATE_NONE, _GATE_FULL, _GATE_GROUP = 0, 1, 2
 _GATE_SIGMOID = 5
@@ -136,15 +138,26 @@ class PackedActivation:
                 f"dtype={self.dtype}, nbytes={self.nbytes})")
 
 
+def _is_nhwc(x: torch.Tensor) -> bool:
+    return (x.dim() == 4
+            and x.is_contiguous(memory_format=torch.channels_last)
+            and not (x.is_contiguous() and x.shape[3] >= x.shape[1]))
+
+
+def _fits(x: torch.Tensor) -> bool:
+    """Whether the codec takes x in one call (2^31 chunks of 8 channels, rows
+    padded to groups; 2^30 channels)."""
+    c = x.shape[1 if _is_nhwc(x) else -1]
+    return c < 1 << 30 and x.numel() // c * -(-c // GROUP) * 4 < 1 << 31
+
+
 def pack_activation(x: torch.Tensor) -> PackedActivation:
     """Keep ``x`` in 8 bits.  Rows are the last axis; of a 4D channels_last
     tensor they are the channels.  (A tensor with one channel or one pixel
     is both: its rows are the longer axis.)"""
     _check_rows(x, "x")
     _check_gpu_dtype(x, "x")
-    nhwc = (x.dim() == 4
-            and x.is_contiguous(memory_format=torch.channels_last)
-            and not (x.is_contiguous() and x.shape[3] >= x.shape[1]))
+    nhwc = _is_nhwc(x)
     rows = x.permute(0, 2, 3, 1) if nhwc else x
     if use_hip(x):
         codes, exps = ext().pack(rows)
@@ -219,8 +232,8 @@ def activations_8bit(min_numel: int = 1 << 16):
     The row operators and ``linear`` run as with ``save8=True``; what any
     other operator saves for its backward pass is packed on saving and
     unpacked on use, if it is a bf16, fp16 or fp32 tensor of two or more
-    axes and at least ``min_numel`` elements and not a weight (see
-    :func:`_is_weight`); that holds for an operator called with
+    axes and at least ``min_numel`` elements, not a weight (see
+    :func:`_is_weight`) and not too large for one call; that holds for an operator called with
     ``save8=False`` too.  Put the model's forward inside and the loss
     outside: what a loss saves are gradients, not activations.  A region
     under ``torch.utils.checkpoint`` is computed again in the backward pass,
@@ -231,7 +244,7 @@ def activations_8bit(min_numel: int = 1 << 16):
 
     def pack(t: torch.Tensor):
         if (t.dtype in _LEAST and t.dim() >= 2 and t.numel() >= min_numel
-                and t.numel() > 0 and not _is_weight(t)):
+                and t.numel() > 0 and _fits(t) and not _is_weight(t)):
             return pack_activation(t)
         return t
 
@@ -351,6 +364,10 @@ def linear8(x: torch.Tensor, weight: torch.Tensor,
                          f"{tuple(weight.shape)}")
     if weight.shape[0] < 1:
         raise ValueError("weight has no outputs")
+    if use_hip(x) and max(weight.shape) > MAX_LINEAR_CHANNELS:
+        raise ValueError(f"an FC layer with save8 takes at most "
+                         f"{MAX_LINEAR_CHANNELS} inputs and outputs, got "
+                         f"{tuple(weight.shape)}")
     if weight.device != x.device:
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
     _param(bias, weight.shape[0], "bias", x)
