@@ -224,3 +224,21 @@ def test_rows_of_more_than_2_to_22_channels(dtype, view):
             ops.linear(x, w, None, save8=True)
     u = ops.row_norm(x[:, 8:1000])  # copied
     assert torch.equal(u, ops.row_norm(x[:, 8:1000].contiguous()))
+
+
+def test_one_row_of_more_than_2_to_29_channels():
+    """More blocks of four chunks than a launch has room for."""
+    c = (1 << 29) + 43
+    z = _rand(1, c, dtype=BF16).view(1, c).requires_grad_()
+    b = torch.full((c,), 0.25, device=DEV, requires_grad=True)
+    dy = torch.ones(1, c, dtype=BF16, device=DEV)
+    y = ops.bias_act(z, b, "relu", save8=True)
+    dz, db = torch.autograd.grad(y, [z, b], dy)
+    del y
+    at = ops.pack_activation(z).unpack()
+    assert torch.equal(dz, ((at.float() + 0.25) > 0).to(BF16))
+    assert torch.equal(db, dz[0].float())
+    del at, z, b, db
+    total = torch.empty((c + 3) // 4 * 4, device=DEV)
+    R.ext().row_sum(dz, total)
+    assert torch.equal(total[:c], dz[0].float())

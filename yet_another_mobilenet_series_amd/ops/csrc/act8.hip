@@ -170,7 +170,7 @@ BwdShape bwd_shape(int64_t rows, int C) {
   BwdShape b;
   const int chunks = ceil_div(C, 8);
   b.TX = 4;
-  if (rows <= 4 * kThreads / b.TX) {
+  if (rows <= 4 * kThreads / b.TX && chunks / b.TX < kMaxBlocks) {
     b.gx = ceil_div(chunks, b.TX);
     b.gy = 1;
     b.per = rows;

@@ -676,7 +676,7 @@ SumShape sum_shape(int64_t rows, int C) {
   SumShape b;
   const int chunks = ceil_div(C, 8);
   b.TX = 4;
-  if (rows <= 16 * 256 / b.TX) {
+  if (rows <= 16 * 256 / b.TX && chunks / b.TX < kMaxBlocks) {
     b.gx = ceil_div(chunks, b.TX);
     b.gy = 1;
     b.per = rows;

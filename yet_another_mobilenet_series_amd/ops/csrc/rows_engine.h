@@ -23,6 +23,10 @@ struct Kept {  // a kept activation; null pointers where there is none
 // bits of bytes (norms and products)
 constexpr int64_t kMaxStride = int64_t(1) << 22;
 
+// blocks of a launch along one axis, at 256 threads: it has fewer than 2^32
+// threads
+constexpr int kMaxBlocks = (1 << 24) - 1;
+
 struct RowsDesc {
   const void* p = nullptr;
   int64_t stride = 0;
