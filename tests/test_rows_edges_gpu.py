@@ -242,3 +242,37 @@ def test_one_row_of_more_than_2_to_29_channels():
     total = torch.empty((c + 3) // 4 * 4, device=DEV)
     R.ext().row_sum(dz, total)
     assert torch.equal(total[:c], dz[0].float())
+
+
+# ---------------------------------------------------------------------------
+# gates
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_sigmoid_gates_have_the_bits_of_fp32(shared):
+    """y = sigmoid(g) and dg = sigmoid'(g).  The exponential and the
+    reciprocal are good to an ulp (2^-23), the correction, the sum and the
+    result to half a one: 2 * 2^-23 + 3 * 2^-24 of the value in all.  For
+    dg, s - s^2, the same of s twice, and a rounding."""
+    c = 2048
+    g = torch.linspace(-87, 30, 4 * c, device=DEV).view(4, c)
+    g[0, :3] = torch.tensor([-float("inf"), float("inf"), float("nan")])
+    g[0, 3:6] = torch.tensor([-1e30, 1e30, 0.0])
+    g.requires_grad_()
+    one = torch.ones((4, 2, c) if shared else (4, c), device=DEV)
+    y = ops.norm_residual(one, torch.zeros_like(one), gate=g,
+                          gate_act="sigmoid", post_norm=False)
+    dg, = torch.autograd.grad(y, g, one)
+    rows = 1
+    if shared:
+        assert torch.equal(y[:, 0].nan_to_num(7.0), y[:, 1].nan_to_num(7.0))
+        y, rows = y[:, 0], 2
+    s = torch.sigmoid(g.detach().double())
+    assert bool(y[0, 2].isnan()) and bool(dg[0, 2].isnan())
+    assert y[0, :2].tolist() == [0.0, 1.0]
+    assert dg[0, [0, 1, 3, 4]].tolist() == [0.0] * 4
+    keep = torch.ones_like(g, dtype=torch.bool)
+    keep[0, 2] = False
+    _within(y[keep], s[keep], 7 * U32 * s[keep], "y")
+    _within(dg[keep], rows * (s * (1 - s))[keep], rows * 15 * U32 * s[keep],
+            "dg")

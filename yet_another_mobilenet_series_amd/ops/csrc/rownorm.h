@@ -153,16 +153,30 @@ DEV_INLINE void row_stats(const float (&v)[NV][8], const int (&n)[NV],
 // Gates.  prepare: what a lane keeps of a gate (sigmoid itself, since its
 // exponential is the expensive part; the other activations' input).
 // value: a(g);  slope: a'(g).  The activation is the same for a launch.
-// v_exp and v_rcp are good to an ulp of fp32.
-template <int NV>
+//
+// 1 / (1 + 2^t), t = -g log2(e).  v_exp and v_rcp are good to an ulp of fp32;
+// rounding t costs |t| / 2 ulps of 2^t, up to 2^-17 of it where that counts,
+// which results of 16 bits do not show.  In fp32 rows 2^t is corrected by what
+// the rounding of t leaves out (where it is neither 0 nor infinite).
+template <int DT, int NV>
 DEV_INLINE void gate_prepare(float (&g)[NV][8], int act) {
+  constexpr float kLog2e = 1.44269502f;      // log2(e) to fp32,
+  constexpr float kLog2eLow = 1.92596299e-8f;  // and what is left
+  constexpr float kLn2 = 0.693147181f;
   if (act == GATE_SIGMOID) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        g[j][e] = __builtin_amdgcn_rcpf(
-            1.f + __builtin_amdgcn_exp2f(-1.44269504f * g[j][e]));
+      for (int e = 0; e < 8; ++e) {
+        const float t = g[j][e] * -kLog2e;
+        float p = __builtin_amdgcn_exp2f(t);
+        if (DT == DT_F32) {
+          const float low = fmaf(g[j][e], -kLog2eLow,
+                                 fmaf(g[j][e], -kLog2e, -t));
+          p = p > 0.f && p < INFINITY ? fmaf(p, low * kLn2, p) : p;
+        }
+        g[j][e] = __builtin_amdgcn_rcpf(1.f + p);
+      }
   }
 }
 

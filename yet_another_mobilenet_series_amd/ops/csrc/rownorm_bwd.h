@@ -280,7 +280,7 @@ join_bwd_kernel(
         q.blank(n[j]);
         decode(q, n[j], gs[j]);
       }
-      gate_prepare<NV>(gs, p.gate_act);
+      gate_prepare<DT, NV>(gs, p.gate_act);
     }
     Raw cur;
     load_row(cur, lo, hi);
@@ -316,7 +316,7 @@ join_bwd_kernel(
           decode(cur.h[j], n[j], h[j]);
           if constexpr (GATE == GATE_FULL) decode(cur.g[j], n[j], g[j]);
         }
-        if constexpr (GATE == GATE_FULL) gate_prepare<NV>(g, p.gate_act);
+        if constexpr (GATE == GATE_FULL) gate_prepare<DT, NV>(g, p.gate_act);
         float mean = 0.f;
         if (p.post)
           row_stats<NV, BT, LAYER>(h, n, TPR, p.inv_c, p.eps, red, turn,

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(BT) void join_fwd_kernel(
       }
     }
     if (HAS_H) {
-      if (GATE != GATE_NONE) gate_prepare<NV>(g, p.gate_act);
+      if (GATE != GATE_NONE) gate_prepare<DT, NV>(g, p.gate_act);
       float mean = 0.f, r = 1.f;
       if (p.post)
         row_stats<NV, BT, LAYER>(h, n, TPR, p.inv_c, p.eps, red, turn, mean,
