@@ -1,6 +1,8 @@
 """Row operators on the CPU: calls that are allowed and rare, and what
 ``activations_8bit`` does with tensors that are no activations."""
 
+import contextlib
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -79,3 +81,188 @@ def test_the_context_leaves_what_the_codec_does_not_take(monkeypatch):
     got, = torch.autograd.grad(y.square().sum(), w)
     want, = torch.autograd.grad(ops.linear(x, w).square().sum(), w)
     assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------
+# weights inside activations_8bit
+# ---------------------------------------------------------------------------
+
+def _grads(run, *wanted, context):
+    """The gradients of run()'s sum of squares' neighbour (a fixed gradient)
+    and the shapes of what was packed."""
+    packed = []
+    pack = R.pack_activation
+
+    def spy(t):
+        packed.append(tuple(t.shape))
+        return pack(t)
+
+    R.pack_activation = spy
+    try:
+        if context:
+            with ops.activations_8bit(min_numel=1):
+                y = run()
+        else:
+            y = run()
+    finally:
+        R.pack_activation = pack
+    dy = torch.linspace(-1, 1, y.numel()).view(y.shape).to(y.dtype)
+    return torch.autograd.grad(y, wanted, dy), packed
+
+
+def _weight(form):
+    """A weight [24, 40] made by `form` from parameters (or none), as a
+    function that a forward pass calls."""
+    torch.manual_seed(6)
+    p = torch.nn.Parameter(torch.randn(24, 40))
+    g = torch.nn.Parameter(torch.rand(24, 1) + 0.5)
+    q = torch.nn.Parameter(torch.randn(40, 24))
+    a, b = (torch.nn.Parameter(torch.randn(*s)) for s in ((24, 5), (5, 40)))
+    mask = (torch.rand(24, 40) > 0.5).float()
+    frozen = torch.nn.Parameter(torch.randn(24, 40), requires_grad=False)
+    conv = torch.nn.Parameter(torch.randn(24, 40, 1, 1))
+    buffer = torch.randn(24, 40)
+    normed = torch.nn.utils.parametrizations.weight_norm(
+        torch.nn.Linear(40, 24, bias=False))
+    return {
+        "parameter": lambda: p,
+        "frozen": lambda: frozen,
+        "frozen, cast": lambda: frozen.double().float(),
+        "frozen, its data": lambda: frozen.data * 1.0,
+        "1x1 filter, viewed and cast":
+            lambda: conv.view(24, 40).double().float(),
+        "transposed copy": lambda: q.t().contiguous(),
+        "weight norm": lambda: g * p / p.norm(dim=1, keepdim=True),
+        "parametrised": lambda: normed.weight,
+        "scaled": lambda: 0.5 * p,
+        "concatenated": lambda: torch.cat([p[:7], frozen[7:]]),
+        "masked": lambda: p * mask,
+        "low rank": lambda: a @ b,
+        "plain": lambda: buffer,
+        "plain, wants a gradient":
+            lambda w=buffer.clone().requires_grad_(): w,
+    }[form]
+
+
+WEIGHTS = ["parameter", "frozen", "frozen, cast", "frozen, its data",
+           "1x1 filter, viewed and cast", "transposed copy", "weight norm",
+           "parametrised", "scaled", "concatenated", "masked", "low rank",
+           "plain", "plain, wants a gradient"]
+
+
+@pytest.mark.parametrize("layer", ["linear", "conv", "matmul", "ops.linear",
+                                   "ops.conv"])
+@pytest.mark.parametrize("form", WEIGHTS)
+def test_weights_are_saved_as_they_are(form, layer):
+    """dx comes from the weight itself, however the weight is made."""
+    weight = _weight(form)
+    x = torch.randn(6, 40, requires_grad=True)
+
+    def run():
+        w, v = weight(), x * 1.0
+        if layer == "linear":
+            return torch.nn.functional.linear(v, w)
+        if layer == "conv":
+            return torch.nn.functional.conv2d(v[:, :, None, None],
+                                              w[:, :, None, None])
+        if layer == "matmul":
+            return v @ w.t()
+        if layer == "ops.linear":
+            return ops.linear(v, w)
+        return ops.conv_bn_act(v[:, :, None, None], w[:, :, None, None],
+                               None, None, None, None)
+
+    (want,), _ = _grads(run, x, context=False)
+    (got,), packed = _grads(run, x, context=True)
+    assert torch.equal(got, want)
+    assert not any(s[:2] in ((24, 40), (40, 24)) for s in packed)
+
+
+@pytest.mark.parametrize("form", ["weight norm", "scaled", "masked"])
+def test_activations_beside_made_weights_are_packed(form):
+    weight = _weight(form)
+    x = torch.randn(6, 40)
+    p = torch.nn.Parameter(torch.randn(24, 24))
+
+    def run():
+        return torch.tanh(x @ weight().t()) @ p
+
+    _, packed = _grads(run, p, context=True)
+    assert packed.count((6, 40)) == 1 and packed.count((6, 24)) >= 1
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+def test_weights_under_autocast(frozen):
+    m = torch.nn.Sequential(torch.nn.Linear(40, 24), torch.nn.Linear(24, 16))
+    m.requires_grad_(not frozen)
+    x = torch.randn(6, 40, requires_grad=True)
+
+    def run():
+        with torch.autocast("cpu", torch.bfloat16):
+            return m(x * 1.0)
+
+    (want,), _ = _grads(run, x, context=False)
+    (got,), packed = _grads(run, x, context=True)
+    assert torch.equal(got, want)
+    assert frozen or set(packed) == {(6, 40), (6, 24)}
+
+
+def test_functional_call_and_attention():
+    m = torch.nn.MultiheadAttention(32, 4, batch_first=True)
+    x = torch.randn(2, 5, 32, requires_grad=True)
+    plain = {k: v.detach().clone() for k, v in m.named_parameters()}
+
+    def run():
+        v = x * 1.0
+        return torch.func.functional_call(m, plain, (v, v, v))[0]
+
+    _, packed = _grads(run, x, context=True)
+    assert packed and not any(s in ((96, 32), (32, 96), (32, 32))
+                              for s in packed)
+
+
+def test_an_input_that_wants_a_gradient_leaves_the_rest_packed():
+    """It is a leaf, and as such like a weight; what follows from it is
+    not."""
+    x = torch.randn(6, 40, requires_grad=True)
+    w = torch.nn.Parameter(torch.randn(24, 40))
+    _, packed = _grads(lambda: torch.tanh(torch.tanh(x) @ w.t()), x,
+                       context=True)
+    assert packed.count((6, 40)) >= 1 and packed.count((6, 24)) == 1
+
+
+def test_nested_contexts_and_threads_know_the_same_weights():
+    import threading
+    weight = _weight("weight norm")
+    x = torch.randn(6, 40, requires_grad=True)
+
+    def run(inner=contextlib.nullcontext):
+        w = weight()
+        with inner():
+            return torch.nn.functional.linear(x * 1.0, w) + (x * 1.0) @ w.t()
+
+    (want,), _ = _grads(run, x, context=False)
+    (got,), _ = _grads(
+        lambda: run(lambda: ops.activations_8bit(min_numel=1)), x,
+        context=True)
+    assert torch.equal(got, want) and not R.saving_8bit()
+    seen = []
+    with ops.activations_8bit():
+        t = threading.Thread(target=lambda: seen.append(R.saving_8bit()))
+        t.start()
+        t.join()
+        assert R.saving_8bit()
+    assert seen == [False]
+
+
+def test_sparse_operands_stay_as_they_are():
+    p = torch.nn.Parameter(torch.randn(40, 24))
+    x = torch.randn(6, 40)
+    adjacency = torch.eye(6).to_sparse()
+
+    def run():
+        return torch.tanh(torch.sparse.mm(adjacency, x @ p))
+
+    (got,), packed = _grads(run, p, context=True)
+    assert set(packed) == {(6, 40), (6, 24)}
+    assert bool(got.isfinite().all())

@@ -276,3 +276,53 @@ def test_sigmoid_gates_have_the_bits_of_fp32(shared):
     _within(y[keep], s[keep], 7 * U32 * s[keep], "y")
     _within(dg[keep], rows * (s * (1 - s))[keep], rows * 15 * U32 * s[keep],
             "dg")
+
+
+# ---------------------------------------------------------------------------
+# weights inside activations_8bit
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("form", ["weight norm", "frozen, cast", "buffer",
+                                  "masked", "transposed copy"])
+def test_linear_in_the_context_uses_the_weight_itself(form):
+    n, k = 72, 264
+    p = torch.nn.Parameter(_rand(1, n, k))
+    q = torch.nn.Parameter(_rand(2, k, n), requires_grad=False)
+    weight = {
+        "weight norm": lambda: p / p.norm(dim=1, keepdim=True),
+        "frozen, cast": lambda: q.t().bfloat16(),
+        "buffer": lambda w=_rand(3, n, k): w,
+        "masked": lambda m=(_rand(4, n, k) > 0).float(): p * m,
+        "transposed copy": lambda: q.t().contiguous()}[form]
+    x = _rand(5, 130, k, dtype=BF16).requires_grad_()
+    dy = _rand(6, 130, n, dtype=BF16)
+    want, = torch.autograd.grad(ops.linear(x * 1.0, weight(), save8=True), x,
+                                dy)
+    with ops.activations_8bit(min_numel=1):
+        y = ops.linear(x * 1.0, weight())
+        z = (x * 1.0) @ weight().to(BF16).t()
+    got, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(got, want)
+    got, = torch.autograd.grad(z, x, dy)
+    want, = torch.autograd.grad((x * 1.0) @ weight().to(BF16).t(), x, dy)
+    assert torch.equal(got, want)
+
+
+def test_the_zoo_keeps_its_weights_and_packs_its_maps(monkeypatch):
+    from yet_another_mobilenet_series_amd import models
+    torch.manual_seed(0)
+    model = models.build_model("mobilenet_v3_small", num_classes=16,
+                               dropout=0.0).to(DEV)
+    model = model.to(memory_format=torch.channels_last).train()
+    packed = []
+    pack = R.pack_activation
+    monkeypatch.setattr(R, "pack_activation",
+                        lambda t: packed.append(tuple(t.shape)) or pack(t))
+    x = _rand(1, 24, 3, 64, 64, dtype=BF16).contiguous(
+        memory_format=torch.channels_last)
+    with ops.activations_8bit(min_numel=1):
+        model(x)
+    weights = {tuple(p.shape) for p in model.parameters()}
+    assert len(packed) > 30
+    assert all(s[0] == 24 for s in packed), [s for s in packed if s[0] != 24]
+    assert not weights.intersection(packed)

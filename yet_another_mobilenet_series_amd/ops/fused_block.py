@@ -30,6 +30,7 @@ import torch
 from .backend import ext
 from .hip_ops import (ACT_IDENTITY, BF16, CL, _empty_like_nhwc, _nhwc,
                       _packed)
+from .rows import with_weights
 
 F32 = torch.float32
 
@@ -438,7 +439,9 @@ def fused_inverted_residual(x, block):
         sw2, sb2 = block.se.fc2.weight, block.se.fc2.bias
     # num_batches_tracked is bumped once per model forward (ZooModel)
     dwm, pjm = block.dw, block.project
-    return FusedInvertedResidualFn.apply(
+    return with_weights(
+        FusedInvertedResidualFn.apply,
+        (ew, dwm.conv.weight, sw1, sw2, pjm.conv.weight),
         x, ew, eg, ebb, erm, erv,
         dwm.conv.weight, dwm.bn.weight, dwm.bn.bias,
         dwm.bn.running_mean, dwm.bn.running_var,

@@ -24,6 +24,7 @@ from typing import Optional, Tuple
 import torch
 
 from .backend import ext
+from .rows import with_weights
 
 BF16 = torch.bfloat16
 CL = torch.channels_last
@@ -296,7 +297,8 @@ def conv_bn_act(x, weight, bn_weight, bn_bias, running_mean, running_var, *,
     else:
         raise NotImplementedError(
             f"conv shape not in the zoo: k={kh} groups={groups} cin={cin_g}")
-    return _ConvBNActFn.apply(
+    return with_weights(
+        _ConvBNActFn.apply, (weight,),
         x, weight, bn_weight, bn_bias, residual, running_mean, running_var,
         kind, kh, stride, padding, act, training, momentum, eps)
 
@@ -349,7 +351,7 @@ class _LinearActFn(torch.autograd.Function):
 
 
 def linear(x, weight, bias=None, act=ACT_IDENTITY):
-    return _LinearActFn.apply(x, weight, bias, act)
+    return with_weights(_LinearActFn.apply, (weight,), x, weight, bias, act)
 
 
 class _GlobalAvgPoolFn(torch.autograd.Function):
@@ -474,7 +476,7 @@ class _SqueezeExciteFn(torch.autograd.Function):
 
 
 def squeeze_excite(x, w1, b1, w2, b2):
-    return _SqueezeExciteFn.apply(x, w1, b1, w2, b2)
+    return with_weights(_SqueezeExciteFn.apply, (w1, w2), x, w1, b1, w2, b2)
 
 
 _dropout_counter = [0]

@@ -38,6 +38,8 @@ from typing import Callable, Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
+from torch.overrides import TorchFunctionMode
+from torch.utils.weak import WeakTensorKeyDictionary
 
 from .backend import ext, use_hip
 
@@ -211,6 +213,121 @@ def _resolve(save8: Optional[bool]) -> bool:
     return saving_8bit() if save8 is None else bool(save8)
 
 
+# Which saved tensors are weights, and stay as they are.  A weight is told by
+# what it is (a parameter) or by how it is used (the weight argument of a
+# layer); a mode that sees torch's calls follows what is made of parameters,
+# and the framework's own layers name their weights (with_weights).
+
+class _Call:
+    """The call that is running: its weights and its other tensors."""
+
+    __slots__ = ("weights", "others", "alone", "casts")
+
+    def __init__(self, weights, others=(), alone=False, casts=True) -> None:
+        self.weights = weights
+        self.others = others  # those that are kept as they are, too
+        self.alone = alone    # a call that makes a weight
+        self.casts = casts    # autocast may have copied them
+
+    def is_weight(self, t: torch.Tensor) -> bool:
+        if self.alone:
+            return True
+        where = t.untyped_storage().data_ptr()
+        return any(
+            w.layout is torch.strided
+            and (w.untyped_storage().data_ptr() == where
+                 or (self.casts and w.numel() == t.numel()
+                     and w.dtype != t.dtype))
+            for group in (self.weights, self.others) for w in group)
+
+
+def with_weights(fn: Callable, weights, *args):
+    """``fn(*args)``, a layer of the framework; inside
+    :func:`activations_8bit` its ``weights`` are saved as they are."""
+    if not saving_8bit():
+        return fn(*args)
+    outer = getattr(_local, "call", None)
+    _local.call = _Call([w for w in weights if w is not None], casts=False)
+    try:
+        with torch._C.DisableTorchFunction():
+            return fn(*args)
+    finally:
+        _local.call = outer
+
+
+#: torch's layers, and where their weight is among the arguments
+_WEIGHT_AT = {"linear": 1, "bilinear": 2, "prelu": 1,
+              **{f"conv{t}{d}d": 1 for d in (1, 2, 3)
+                 for t in ("", "_transpose")}}
+#: products, of which a tensor without a graph is an operand like a weight
+_PRODUCTS = {*_WEIGHT_AT, "matmul", "__matmul__", "__rmatmul__", "mm", "bmm",
+             "addmm", "baddbmm", "addbmm", "einsum", "tensordot", "mv",
+             "inner", "outer", "multi_head_attention_forward"}
+#: what a plain tensor, no larger than it, does to a weight: masking it
+_MASKS = {"mul", "__mul__", "__rmul__", "where", "masked_fill"}
+
+
+class _WeightsMode(TorchFunctionMode):
+    """Sees the calls inside :func:`activations_8bit` and tells the saved
+    tensors that are weights from the others."""
+
+    def __init__(self) -> None:
+        super().__init__()
+        self.made = WeakTensorKeyDictionary()  # of parameters alone
+
+    def of_parameters(self, t: torch.Tensor) -> bool:
+        base = t if t._base is None else t._base
+        return (isinstance(base, torch.nn.Parameter)
+                or isinstance(t, torch.nn.Parameter)
+                or (len(self.made) > 0
+                    and (t in self.made or base in self.made)))
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        kwargs = kwargs or {}
+        name = getattr(func, "__name__", "")
+        if name == "__get__":
+            out = func(*args, **kwargs)
+            if isinstance(out, torch.Tensor) and self.of_parameters(args[0]):
+                self.made[out] = True  # W.data
+            return out
+        tensors = []
+        for a in (*args, *kwargs.values()):
+            if isinstance(a, torch.Tensor):
+                tensors.append(a)
+            elif isinstance(a, (list, tuple)):
+                tensors += [t for t in a if isinstance(t, torch.Tensor)]
+        if not tensors:
+            return func(*args, **kwargs)
+        params = [self.of_parameters(t) for t in tensors]
+        at, used = _WEIGHT_AT.get(name), None
+        if at is not None:
+            used = kwargs.get("weight", args[at] if at < len(args) else None)
+        weights, rest = [], []
+        for t, p in zip(tensors, params):
+            (weights if p or t is used or _is_weight(t) else rest).append(t)
+        # a tensor without a graph beside one that has it: a coefficient of
+        # a product, or one that is broadcast
+        most = max((t.numel() for t in rest if t.requires_grad), default=-1)
+        plain = [t for t in rest if not t.requires_grad and most >= 0
+                 and (name in _PRODUCTS or t.numel() < most)]
+        alone = all(params) or (
+            name in _MASKS and any(params)
+            and not any(t.requires_grad for t in rest)
+            and max(t.numel() for t in weights)
+            >= max((t.numel() for t in rest), default=0))
+        outer = getattr(_local, "call", None)
+        _local.call = _Call(weights, plain, alone)
+        try:
+            out = func(*args, **kwargs)
+        finally:
+            _local.call = outer
+        if alone:
+            for t in out if isinstance(out, (list, tuple)) else (out,):
+                if isinstance(t, torch.Tensor):
+                    self.made[t] = True
+        return out
+
+
 def _is_weight(t: torch.Tensor) -> bool:
     """A parameter (frozen or not), another leaf that wants a gradient, what
     a single operator (a cast) made of a parameter that wants one, or a view
@@ -231,32 +348,61 @@ def activations_8bit(min_numel: int = 1 << 16):
 
     The row operators and ``linear`` run as with ``save8=True``; what any
     other operator saves for its backward pass is packed on saving and
-    unpacked on use, if it is a bf16, fp16 or fp32 tensor of two or more
-    axes and at least ``min_numel`` elements, not a weight (see
-    :func:`_is_weight`) and not too large for one call; that holds for an operator called with
-    ``save8=False`` too.  Put the model's forward inside and the loss
-    outside: what a loss saves are gradients, not activations.  A region
-    under ``torch.utils.checkpoint`` is computed again in the backward pass,
-    outside: pass ``save8`` to the operators in it (a region that is not
-    computed again as it was raises an error there)."""
+    unpacked on use, if it is a dense bf16, fp16 or fp32 tensor of two or more
+    axes and at least ``min_numel`` elements, not a weight and not too large
+    for one call; that holds for an operator called with ``save8=False``
+    too.  Put the model's forward inside and the loss outside: what a loss
+    saves are gradients, not activations.
+
+    Weights are: parameters, frozen or not, and other leaves that want a
+    gradient; views of these; what is made inside from parameters alone, by
+    any number of operators, and from a parameter and a mask;
+    the weight argument of a layer (this framework's, torch's linear,
+    bilinear, prelu and convolutions), whatever tensor it is; and a tensor
+    without a graph that is multiplied with one that has it (a buffer).
+    Anything else, as a weight made before the context and handed to
+    ``matmul``, or to an autograd function of your own, is an activation.
+
+    Small values of a group become zero.  An operator that divides by what
+    it saves, as ``log``, ``sqrt`` and division do, then has infinite
+    gradients there: keep such operators outside.
+
+    Each operator keeps codes of its own, 1 + 1/32 bytes a value.  A tensor
+    that several operators save costs that for each of them, where it would
+    otherwise be saved once (2 bytes a value in bf16).
+
+    A region under ``torch.utils.checkpoint`` is computed again in the
+    backward pass, outside: pass ``save8`` to the operators in it (a region
+    that is not computed again as it was raises an error there)."""
     if min_numel < 0:
         raise ValueError(f"min_numel must not be negative, got {min_numel}")
 
+    outer = getattr(_local, "mode", None)
+    mode = _WeightsMode() if outer is None else outer
+
     def pack(t: torch.Tensor):
-        if (t.dtype in _LEAST and t.dim() >= 2 and t.numel() >= min_numel
-                and t.numel() > 0 and _fits(t) and not _is_weight(t)):
-            return pack_activation(t)
-        return t
+        with torch._C.DisableTorchFunction():
+            if (t.dtype not in _LEAST or t.layout is not torch.strided
+                    or t.dim() < 2 or t.numel() == 0
+                    or t.numel() < min_numel or not _fits(t)
+                    or _is_weight(t) or mode.of_parameters(t)):
+                return t
+            call = getattr(_local, "call", None)
+            return (t if call is not None and call.is_weight(t)
+                    else pack_activation(t))
 
     def unpack(kept):
         return kept.unpack() if isinstance(kept, PackedActivation) else kept
 
-    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+    with (mode if outer is None else contextlib.nullcontext()), \
+            torch.autograd.graph.saved_tensors_hooks(pack, unpack):
         _local.depth = getattr(_local, "depth", 0) + 1
+        _local.mode = mode
         try:
             yield
         finally:
             _local.depth -= 1
+            _local.mode = outer
 
 
 class _Keep8Fn(torch.autograd.Function):
@@ -372,11 +518,13 @@ def linear8(x: torch.Tensor, weight: torch.Tensor,
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
     _param(bias, weight.shape[0], "bias", x)
     if use_hip(x):
-        z = ext().linear8(x, weight, bias if act == 0 else None)
+        z = with_weights(ext().linear8, (weight,), x, weight,
+                         bias if act == 0 else None)
     else:
-        z = _reference(lambda x, w, b: F.linear(x, w, b),
-                       (True, False, False), save8, x, weight,
-                       bias if act == 0 else None)
+        z = with_weights(_reference, (weight,),
+                         lambda x, w, b: F.linear(x, w, b),
+                         (True, False, False), save8, x, weight,
+                         bias if act == 0 else None)
     return z if act == 0 else bias_act(z, bias, act, save8)
 
 
