@@ -266,3 +266,29 @@ def test_sparse_operands_stay_as_they_are():
     (got,), packed = _grads(run, p, context=True)
     assert set(packed) == {(6, 40), (6, 24)}
     assert bool(got.isfinite().all())
+
+
+# ---------------------------------------------------------------------------
+# gradients that divide by what is saved
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fn", [
+    torch.log, torch.sqrt, torch.log1p, lambda v: v ** 0.5, lambda v: 1 / v,
+    lambda v: v / v.flip(0), lambda v: torch.nn.functional.normalize(v, dim=0),
+    lambda v: v.std(0), lambda v: torch.linalg.vector_norm(v, dim=1),
+    lambda v: v.norm(dim=1), lambda v: torch.div(2.0, v)],
+    ids="log sqrt log1p pow reciprocal div normalize std vector_norm norm "
+        "torch.div".split())
+def test_finite_gradients_stay_finite(fn):
+    """Positive maps with values below a unit of their group."""
+    torch.manual_seed(7)
+    x = torch.rand(64, 64).pow(8) + 1e-12
+    x.requires_grad_()
+
+    def run():
+        return fn(x * 1.0)
+
+    (want,), _ = _grads(run, x, context=False)
+    (got,), _ = _grads(run, x, context=True)
+    assert bool(want.isfinite().all())
+    assert torch.equal(got, want)

@@ -221,16 +221,16 @@ def _resolve(save8: Optional[bool]) -> bool:
 class _Call:
     """The call that is running: its weights and its other tensors."""
 
-    __slots__ = ("weights", "others", "alone", "casts")
+    __slots__ = ("weights", "others", "all", "casts")
 
-    def __init__(self, weights, others=(), alone=False, casts=True) -> None:
+    def __init__(self, weights, others=(), all=False, casts=True) -> None:
         self.weights = weights
         self.others = others  # those that are kept as they are, too
-        self.alone = alone    # a call that makes a weight
+        self.all = all        # everything is: it makes a weight, or divides
         self.casts = casts    # autocast may have copied them
 
-    def is_weight(self, t: torch.Tensor) -> bool:
-        if self.alone:
+    def keeps(self, t: torch.Tensor) -> bool:
+        if self.all:
             return True
         where = t.untyped_storage().data_ptr()
         return any(
@@ -263,6 +263,15 @@ _WEIGHT_AT = {"linear": 1, "bilinear": 2, "prelu": 1,
 _PRODUCTS = {*_WEIGHT_AT, "matmul", "__matmul__", "__rmatmul__", "mm", "bmm",
              "addmm", "baddbmm", "addbmm", "einsum", "tensordot", "mv",
              "inner", "outer", "multi_head_attention_forward"}
+#: what divides by the tensors it saves: small values of a group become zero,
+#: and a finite gradient infinite
+_DIVIDES = {"div", "div_", "divide", "true_divide", "__truediv__", "__idiv__",
+            "__itruediv__", "__rdiv__", "__rtruediv__", "reciprocal", "log",
+            "log2", "log10", "log1p", "xlogy", "logit", "sqrt", "pow",
+            "__pow__", "__rpow__", "float_power", "norm", "vector_norm",
+            "linalg_vector_norm", "normalize", "cosine_similarity", "std",
+            "std_mean", "prod", "cumprod", "atan2", "acosh", "asinh",
+            "lgamma", "digamma"}
 #: what a plain tensor, no larger than it, does to a weight: masking it
 _MASKS = {"mul", "__mul__", "__rmul__", "where", "masked_fill"}
 
@@ -316,7 +325,7 @@ class _WeightsMode(TorchFunctionMode):
             and max(t.numel() for t in weights)
             >= max((t.numel() for t in rest), default=0))
         outer = getattr(_local, "call", None)
-        _local.call = _Call(weights, plain, alone)
+        _local.call = _Call(weights, plain, alone or name in _DIVIDES)
         try:
             out = func(*args, **kwargs)
         finally:
@@ -348,24 +357,25 @@ def activations_8bit(min_numel: int = 1 << 16):
 
     The row operators and ``linear`` run as with ``save8=True``; what any
     other operator saves for its backward pass is packed on saving and
-    unpacked on use, if it is a dense bf16, fp16 or fp32 tensor of two or more
-    axes and at least ``min_numel`` elements, not a weight and not too large
-    for one call; that holds for an operator called with ``save8=False``
-    too.  Put the model's forward inside and the loss outside: what a loss
+    unpacked on use, if it is a dense bf16, fp16 or fp32 tensor of two or
+    more axes and at least ``min_numel`` elements, not a weight and not too
+    large for one call; that holds for an operator called with
+    ``save8=False`` too.  Put the model's forward inside and the loss outside: what a loss
     saves are gradients, not activations.
 
     Weights are: parameters, frozen or not, and other leaves that want a
     gradient; views of these; what is made inside from parameters alone, by
-    any number of operators, and from a parameter and a mask;
-    the weight argument of a layer (this framework's, torch's linear,
-    bilinear, prelu and convolutions), whatever tensor it is; and a tensor
-    without a graph that is multiplied with one that has it (a buffer).
+    any number of operators, and from a parameter and a mask; the weight
+    argument of a layer (this framework's, torch's linear, bilinear, prelu
+    and convolutions), whatever tensor it is; and a tensor without a graph
+    that is multiplied with one that has it (a buffer).
     Anything else, as a weight made before the context and handed to
     ``matmul``, or to an autograd function of your own, is an activation.
 
-    Small values of a group become zero.  An operator that divides by what
-    it saves, as ``log``, ``sqrt`` and division do, then has infinite
-    gradients there: keep such operators outside.
+    Small values of a group become zero, and a gradient that divides by them
+    infinite.  Torch's operators that do so (division, ``log``, ``sqrt``,
+    powers, norms and the like) are therefore left alone; an autograd function
+    of your own that does belongs outside.
 
     Each operator keeps codes of its own, 1 + 1/32 bytes a value.  A tensor
     that several operators save costs that for each of them, where it would
@@ -388,7 +398,7 @@ def activations_8bit(min_numel: int = 1 << 16):
                     or _is_weight(t) or mode.of_parameters(t)):
                 return t
             call = getattr(_local, "call", None)
-            return (t if call is not None and call.is_weight(t)
+            return (t if call is not None and call.keeps(t)
                     else pack_activation(t))
 
     def unpack(kept):
