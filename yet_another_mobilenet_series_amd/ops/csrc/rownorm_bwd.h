@@ -243,13 +243,14 @@ join_bwd_kernel(
     }
   };
 
-  // `n_` (0..8) of the chunk's values, and zeros: what lies behind the last
-  // channel has code 0, which is NaN in a group with a non-finite value
-  auto decode = [&](const RawChunk<DT, KEPT>& q, int n_, float* v) {
-    q.decode(v);
+  // zeros behind the last channel: it has code 0 there, which is NaN in a
+  // group with a non-finite value
+  auto end_row = [&](float (&v)[NV][8]) {
     if (KEPT && p.read != READ_WHOLE) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n_ ? v[e] : 0.f;
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = e < n[j] ? v[j][e] : 0.f;
     }
   };
 
@@ -278,8 +279,9 @@ join_bwd_kernel(
              p.read == READ_SHORT ? n[j] : -1);
         if (p.read == READ_RAGGED) q.drop(n[j]);
         q.blank(n[j]);
-        decode(q, n[j], gs[j]);
+        q.decode(gs[j]);
       }
+      if constexpr (KEPT) end_row(gs);
       gate_prepare<DT, NV>(gs, p.gate_act);
     }
     Raw cur;
@@ -313,8 +315,12 @@ join_bwd_kernel(
       if constexpr (HAS_H) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          decode(cur.h[j], n[j], h[j]);
-          if constexpr (GATE == GATE_FULL) decode(cur.g[j], n[j], g[j]);
+          cur.h[j].decode(h[j]);
+          if constexpr (GATE == GATE_FULL) cur.g[j].decode(g[j]);
+        }
+        if (KEPT && p.read != READ_WHOLE) {
+          end_row(h);
+          if constexpr (GATE == GATE_FULL) end_row(g);
         }
         if constexpr (GATE == GATE_FULL) gate_prepare<DT, NV>(g, p.gate_act);
         float mean = 0.f;
@@ -330,8 +336,10 @@ join_bwd_kernel(
       }
       if (next) {
 #pragma unroll
+        for (int j = 0; j < NV; ++j) cur.x[j].decode(x[j]);
+        end_row(x);
+#pragma unroll
         for (int j = 0; j < NV; ++j) {
-          decode(cur.x[j], n[j], x[j]);
           if constexpr (HAS_H) {
             float w[8], s[8], b[8] = {};
             pw.get(p.w, t + j * TPR, n[j], 1.f, 1.f, w);
