@@ -326,3 +326,33 @@ def test_the_zoo_keeps_its_weights_and_packs_its_maps(monkeypatch):
     assert len(packed) > 30
     assert all(s[0] == 24 for s in packed), [s for s in packed if s[0] != 24]
     assert not weights.intersection(packed)
+
+
+@pytest.mark.parametrize("shape", [
+    (512, 3, 16), (600, 1, 8), (700, 2, 40), (3, 65, 16), (90, 63, 24),
+    (1, 3, 16), (1000, 5, 333), (2000, 2, 1500)])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_gates_of_short_runs(shape, kind):
+    """The sums over short runs, and over many of them, are those of a gate
+    for every row: the same terms in another order."""
+    n, m, c = shape
+    h, x = _rand(1, *shape), _rand(2, *shape)
+    g, s = _rand(3, n, c).requires_grad_(), _rand(4, c).requires_grad_()
+    w = _rand(5, c).requires_grad_()
+    dy, du = _rand(6, *shape), _rand(7, *shape)
+
+    def grads(gate):
+        outs = ops.norm_residual(h, x, w, gate=gate, gate_act="sigmoid",
+                                 scale=s, next_norm=True, kind=kind)
+        return outs + torch.autograd.grad(outs, [gate, s, w], [dy, du])
+
+    y, u, dg, ds, dw = grads(g)
+    full = g.detach()[:, None].expand(shape).contiguous().requires_grad_()
+    y1, u1, dg1, ds1, dw1 = grads(full)
+    assert torch.equal(y, y1) and torch.equal(u, u1)
+    # the terms are the same bits, their sums in fp32
+    _within(dg, dg1.double().sum(1), m * U32 * dg1.double().abs().sum(1))
+    for p, q in ((ds, ds1), (dw, dw1)):
+        # at most a few units a term, each a product of a handful of these
+        off = (p.double() - q.double()).abs().max()
+        assert float(off) <= 256 * U32 * 64 * n * m

@@ -68,14 +68,18 @@ BwdPlan bwd_plan(int dt, const JoinDesc& d) {
   // the blocks that the chip holds at once, by the registers of the kernels
   // (bwd_waves(); two waves a SIMD for fp32 with what LayerNorm and a gate
   // take: 20000 x 1536 318 -> 254 us with 512 blocks for 768); fewer where a
-  // team would get under four rows
+  // block would get under four steps.  Runs shorter than a step leave teams
+  // idle, so that they get blocks of their own (512 runs of 3 x 16: 915 us
+  // with 6 blocks, 9.5 with 512).
   const bool has_h = d.h.p != nullptr || d.hk.codes != nullptr;
   const bool four = b.r.BT >= 512 || !has_h ||
                     (!d.layer && dt != DT_F32 && !shared);
   const bool two = dt == DT_F32 && d.layer && d.gate != GATE_NONE;
   const int64_t most = 256 * (four ? 1024 : two ? 512 : 768) / b.r.BT;
-  const int64_t blocks = std::max<int64_t>(
-      1, std::min<int64_t>(most, d.rows / (4 * rpb)));
+  const int64_t steps = b.groups * ((b.group_rows + rpb - 1) / rpb);
+  const int64_t blocks = std::min<int64_t>(
+      most, std::max<int64_t>({1, steps / 4,
+                               b.group_rows < rpb ? b.groups : 0}));
   if (b.groups >= blocks) {
     b.parts = 1;
     b.part_rows = b.group_rows;

@@ -218,12 +218,13 @@ join_bwd_kernel(
       load_rows(q, base, live, false);
   };
 
-  // adds a per-channel sum over the teams of the block; the result is in
-  // the first team's registers (team by team: eight values in flight, and
-  // not registers for all of them)
+  // adds a per-channel sum over the teams of the block that may have had a
+  // row; the result is in the first team's registers (team by team: eight
+  // values in flight, and not registers for all of them)
+  const int teams = int(min(p.part_rows, int64_t(RPB)));
   auto over_teams = [&](float (&v)[NV][8]) {
     if constexpr (BT <= 256) {
-      if (RPB > 1) {
+      if (teams > 1) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           __syncthreads();
@@ -233,7 +234,7 @@ join_bwd_kernel(
           __syncthreads();
           if (team == 0) {
 #pragma unroll 1
-            for (int l = 1; l < RPB; ++l)
+            for (int l = 1; l < teams; ++l)
 #pragma unroll
               for (int e = 0; e < 8; ++e)
                 v[j][e] += fold[e * BT + l * TPR + t];
