@@ -74,6 +74,12 @@ def test_the_context_leaves_what_the_codec_does_not_take(monkeypatch):
     want, = torch.autograd.grad(torch.tanh(x @ w).sum(), w)
     assert torch.equal(got, want)
 
+    w16 = one.expand(16, 1024)
+    assert R.linear_fits(one.expand((1 << 24) - 1, 1024), w16)
+    assert not R.linear_fits(one.expand(1 << 24, 1024), w16)
+    assert not R.linear_fits(one.expand(1 << 20, 64), one.expand(1 << 17, 64))
+    assert not R.linear_fits(one.expand(2, (1 << 22) + 1),
+                             one.expand(1, (1 << 22) + 1))
     monkeypatch.setattr(R, "MAX_LINEAR_CHANNELS", 32)
     x = x.requires_grad_()
     with ops.activations_8bit(min_numel=1):

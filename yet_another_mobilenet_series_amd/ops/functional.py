@@ -207,8 +207,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor,
     bits (:mod:`.rows`; default: as ``activations_8bit`` says, for layers
     of the size that ``save8`` takes)."""
     if save8 is None:
-        save8 = (rows.saving_8bit()
-                 and max(weight.shape) <= rows.MAX_LINEAR_CHANNELS)
+        save8 = rows.saving_8bit() and rows.linear_fits(x, weight)
     if save8:
         return rows.linear8(x, weight, bias, act_code(act))
     if use_hip(x):

@@ -504,6 +504,19 @@ def bias_act(z: torch.Tensor, bias: Optional[torch.Tensor] = None,
 # FC layer on an input kept in 8 bits
 # ---------------------------------------------------------------------------
 
+def linear_fits(x: torch.Tensor, weight: torch.Tensor) -> bool:
+    """Whether :func:`linear8` takes a layer of this size: its channels, the
+    codec's chunks, and 2^24 tiles of 64 x 64 for each of its products."""
+    if weight.dim() != 2 or weight.numel() == 0:
+        return True  # refused by name
+    n, k = weight.shape
+    m = x.numel() // k
+    t = [-(-v // 64) for v in (m, n, k)]
+    return (max(n, k) <= MAX_LINEAR_CHANNELS
+            and m * -(-k // GROUP) * 4 < 1 << 31
+            and max(t[0] * t[1], t[0] * t[2], t[1] * t[2]) < 1 << 24)
+
+
 def linear8(x: torch.Tensor, weight: torch.Tensor,
             bias: Optional[torch.Tensor], act: int,
             save8: bool = True) -> torch.Tensor:
