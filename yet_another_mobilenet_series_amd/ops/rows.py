@@ -33,6 +33,7 @@ autograd_rows.cpp), CPU tensors and
 from __future__ import annotations
 
 import contextlib
+import functools
 import threading
 from typing import Callable, Optional, Tuple, Union
 
@@ -255,6 +256,19 @@ def with_weights(fn: Callable, weights, *args):
         _local.call = outer
 
 
+def _unwatched(fn: Callable) -> Callable:
+    """An operator of this module: the mode of :func:`activations_8bit` has
+    nothing to see in it, and would see every attribute that it checks (some
+    25 of a join, 2 us each)."""
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        if not saving_8bit():
+            return fn(*args, **kwargs)
+        with torch._C.DisableTorchFunction():
+            return fn(*args, **kwargs)
+    return call
+
+
 #: torch's layers, and where their weight is among the arguments
 _WEIGHT_AT = {"linear": 1, "bilinear": 2, "prelu": 1,
               **{f"conv{t}{d}d": 1 for d in (1, 2, 3)
@@ -473,6 +487,7 @@ def _up(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 # bias + activation
 # ---------------------------------------------------------------------------
 
+@_unwatched
 def bias_act(z: torch.Tensor, bias: Optional[torch.Tensor] = None,
              act: Union[int, str] = 0, save8: Optional[bool] = None
              ) -> torch.Tensor:
@@ -517,6 +532,7 @@ def linear_fits(x: torch.Tensor, weight: torch.Tensor) -> bool:
             and max(t[0] * t[1], t[0] * t[2], t[1] * t[2]) < 1 << 24)
 
 
+@_unwatched
 def linear8(x: torch.Tensor, weight: torch.Tensor,
             bias: Optional[torch.Tensor], act: int,
             save8: bool = True) -> torch.Tensor:
@@ -583,6 +599,7 @@ def _check_norm_rows(x: torch.Tensor, name: str) -> None:
                              f"channels, got {x.shape[-1]}")
 
 
+@_unwatched
 def row_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
              bias: Optional[torch.Tensor] = None, *, kind: str = "rms",
              eps: float = 1e-6, save8: Optional[bool] = None
@@ -620,6 +637,7 @@ def _gate_code(name: str) -> int:
                          f"{name!r}") from None
 
 
+@_unwatched
 def norm_residual(
     h: torch.Tensor, x: torch.Tensor,
     weight: Optional[torch.Tensor] = None,
