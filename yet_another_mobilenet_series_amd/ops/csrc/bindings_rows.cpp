@@ -404,7 +404,8 @@ void linear8_wgrad(const Tensor& dy, const Tensor& codes, const Tensor& exps,
                      exps.data_ptr<uint8_t>()};
   const bool padded =
       int64_t(codes.storage().nbytes()) - codes.storage_offset() >= M * K + 7;
-  Tensor ws = cy.ws(yams::linear8_ws(cy.C, K, M, kBf16));
+  Tensor ws = cy.ws(yams::linear8_ws(cy.C, K, M, kBf16,
+                                     yams::linear8_loose(K, padded)));
   yams::linear8_wgrad(cy.in(dy, "dy"), x, padded, odt, dw.data_ptr(),
                       ws_ptr(ws), M, cy.C, int(K), stream_of(dy));
 }

@@ -697,16 +697,16 @@ Operand operand(RowsDesc r) { return {r.p, r.stride, nullptr, 0}; }
 
 }  // namespace
 
-int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth, int wdt) {
+int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth, int wdt,
+                   bool loose) {
   if (rows == 0 || cols == 0 || depth == 0) return 0;
-  int64_t most = 0;  // of the two plans that the product may have
-  for (const bool loose : {false, true}) {
-    const int splits =
-        plan_of(rows, cols, depth, wdt == DT_F32 ? 2 : 1, loose).splits;
-    if (splits > 1) most = std::max(most, splits * rows * cols);
-  }
-  return most;
+  const int splits =
+      plan_of(rows, cols, depth, wdt == DT_F32 ? 2 : 1, loose).splits;
+  return splits > 1 ? splits * rows * cols : 0;
 }
+
+// codes of a width that is no multiple of 8 are read up to seven behind a row
+bool linear8_loose(int64_t K, bool padded) { return K % 8 != 0 && !padded; }
 
 void linear8_fwd(RowsDesc x, int wdt, RowsDesc w, int bdt, const void* b,
                  void* y, float* ws, int64_t M, int N, int K, hipStream_t s) {
@@ -736,7 +736,7 @@ void linear8_wgrad(RowsDesc dy, Kept x, bool padded, int odt, void* dw,
   if (N == 0 || K == 0) return;
   Operand b{x.codes, K, x.exps, ceil_div(K, kGroup)};
   product<OP_BF16, true, OP_CODE, true>(operand(dy), b, odt, dw, Bias{}, ws,
-                                        N, K, M, K % 8 != 0 && !padded, s);
+                                        N, K, M, linear8_loose(K, padded), s);
 }
 
 int64_t row_sum_ws(int64_t rows, int C) {

@@ -103,8 +103,11 @@ void linear8_dgrad(RowsDesc dy, int wdt, RowsDesc w, void* dx, float* ws,
 void linear8_wgrad(RowsDesc dy, Kept x, bool padded, int odt, void* dw,
                    float* ws, int64_t M, int N, int K, hipStream_t s);
 // floats of `ws` for [rows, cols] outputs over a reduction of `depth`; `wdt`
-// of the weights (the weight gradient has codes in their place: DT_BF16)
-int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth, int wdt);
+// of the weights (the weight gradient has codes in their place: DT_BF16, and
+// says whether they are `loose`)
+int64_t linear8_ws(int64_t rows, int64_t cols, int64_t depth, int wdt,
+                   bool loose = false);
+bool linear8_loose(int64_t K, bool padded);
 // db = sum over rows of dy; ws of row_sum_ws floats; db as dbias above
 // (`odt` DT_F32) or bf16 [C] (DT_BF16)
 void row_sum(int dt, RowsDesc dy, int odt, void* db, float* ws, int64_t rows,
