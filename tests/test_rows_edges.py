@@ -298,3 +298,33 @@ def test_finite_gradients_stay_finite(fn):
     (got,), _ = _grads(run, x, context=True)
     assert bool(want.isfinite().all())
     assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------
+# layouts
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("op", ["row_norm", "bias_act", "norm_residual",
+                                "linear"])
+def test_rows_are_the_last_axis_in_any_layout(op):
+    """A 4D tensor whose memory happens to be that of a channels_last map:
+    its rows are kept, not its second axis."""
+    torch.manual_seed(8)
+    x = torch.randn(40, 1, 6, 5).permute(1, 2, 3, 0) * torch.arange(1.0, 41)
+    x = x.contiguous(memory_format=torch.channels_last)
+    assert x.is_contiguous(memory_format=torch.channels_last)
+    dy = torch.randn(x.shape)
+    w = torch.randn(40, 40)
+
+    def grad(v):
+        v = v.detach().requires_grad_()
+        s = torch.ones(40, requires_grad=True)
+        y = {"row_norm": lambda: ops.row_norm(v, s, save8=True),
+             "bias_act": lambda: ops.bias_act(v, s, "hswish", save8=True),
+             "norm_residual": lambda: ops.norm_residual(
+                 v, v, scale=s, gate=v, next_norm=True, save8=True)[1],
+             "linear": lambda: ops.linear(v, w * s, None, save8=True)}[op]()
+        return torch.autograd.grad(y, [v, s], dy)
+
+    for a, b in zip(grad(x), grad(x.contiguous())):
+        assert torch.equal(a, b)

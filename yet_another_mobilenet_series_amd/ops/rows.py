@@ -440,9 +440,11 @@ class _Keep8Fn(torch.autograd.Function):
         saved, ctx.form = [], []
         for t, k in zip(tensors, kept):
             if t is not None and k:
-                p = pack_activation(t)
-                saved += [p.codes, p.exponents]
-                ctx.form.append((p.shape, p.dtype, p.nhwc))
+                # by rows, whatever the layout: not as pack_activation, which
+                # takes the channels of a channels_last map
+                _check_gpu_dtype(t, "what is kept in 8 bits")
+                saved += _ref_pack(_rows(t.detach()))
+                ctx.form.append((t.shape, t.dtype))
             else:
                 saved.append(t)
                 ctx.form.append(None)
